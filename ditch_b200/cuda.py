@@ -74,6 +74,32 @@ class Params(C.Structure):
                 ("min_weight_distance", C.c_float)]
 
 
+class KvCacheDesc(C.Structure):
+    _fields_ = [("format", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int),
+                ("block_tokens", C.c_int), ("n_pages", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class KvBatchDesc(C.Structure):
+    _fields_ = [("n_seqs", C.c_size_t), ("n_tokens", C.c_size_t), ("max_new", C.c_size_t), ("max_len", C.c_size_t),
+                ("max_pages", C.c_size_t), ("offsets", C.c_void_p), ("lens", C.c_void_p), ("pages", C.c_void_p)]
+
+
+class RowsDesc(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("heads", C.c_int), ("token_stride", C.c_size_t),
+                ("head_stride", C.c_size_t)]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("table_len", C.c_size_t), ("half", C.c_size_t),
+                ("style", C.c_int)]
+
+
+class RaggedDesc(C.Structure):
+    _fields_ = [("n_seqs", C.c_size_t), ("n_q", C.c_size_t), ("n_kv", C.c_size_t), ("max_q", C.c_size_t),
+                ("max_kv", C.c_size_t), ("q_offsets", C.c_void_p), ("kv_offsets", C.c_void_p)]
+
+
 _lib = None
 vp, sz, f32p, f64p, u8p, u16p, u32p, u64p = (C.c_void_p, C.c_size_t, C.POINTER(C.c_float), C.POINTER(C.c_double),
                                              C.POINTER(C.c_uint8), C.POINTER(C.c_uint16), C.POINTER(C.c_uint32),
@@ -129,6 +155,11 @@ SIGNATURES = {
     "ditch_cuda_kl_score_prompts": (C.c_int, [vp, u32p, C.POINTER(sz), sz, f64p]),
     "ditch_cuda_edit_weight_bf16": (C.c_int, [vp, vp, sz, sz, vp, C.c_float]),
     "ditch_cuda_edit_weight_bf16_noalloc": (C.c_int, [vp, sz, sz, vp, C.c_float, vp]),
+    "ditch_cuda_kv_append": (C.c_int, [vp] * 11),
+    "ditch_cuda_kv_read": (C.c_int, [vp] * 6),
+    "ditch_cuda_kv_attention_workspace": (sz, [vp, vp, vp, sz]),
+    "ditch_cuda_kv_attention": (C.c_int, [vp] * 5 + [C.c_float, sz, sz, vp, sz, vp]),
+    "ditch_cuda_window_attention": (C.c_int, [vp, vp, sz, vp, vp, vp, vp, C.c_float, sz, sz, vp]),
     "ditch_cuda_weight_load": (C.c_int, [vp, C.POINTER(TensorDesc), C.POINTER(vp)]),
     "ditch_cuda_weight_free": (None, [vp]),
     "ditch_cuda_weight_format": (C.c_int, [vp]),
@@ -190,6 +221,11 @@ def _p(a, t):
         return None
     assert a.flags["C_CONTIGUOUS"]
     return a.ctypes.data_as(t)
+
+
+def _dev(t):
+    """The device address of a tensor (anything with data_ptr()) or of an int."""
+    return None if t is None else t.data_ptr() if hasattr(t, "data_ptr") else int(t)
 
 
 def _f32(a):
@@ -312,6 +348,14 @@ class Device:
         check(lib().ditch_cuda_rope_rows(self.h, _p(x, f32p), n, dim, _p(c, f32p), _p(s, f32p), c.shape[0],
                                          c.shape[1], _p(pos, u32p), style))
         return x
+
+    def window_attention(self, ragged, q, k, v, out, head_dim, scale, window=0, sinks=0, stream=0):
+        """Causal attention over contiguous device rows (f16 or bf16), with a
+        sliding window and sinks (ditch_cuda_window_attention)."""
+        st = lib().ditch_cuda_window_attention(self.h, ragged.ref, head_dim, q.ref, k.ref, v.ref, out.ref, scale,
+                                               window, sinks, stream)
+        if st:
+            check(st)
 
     # ---- decoders ----
     def dequant_fp8(self, codes, scales, br, bc):
@@ -485,6 +529,98 @@ class Weight:
             self.close()
         except Exception:
             pass
+
+
+class _Desc:
+    """A C descriptor built once; `ref` is the pointer the entries take, `keep`
+    the tensors it points into."""
+
+    def __init__(self, desc, *keep):
+        self.desc = desc
+        self.ref = C.cast(C.pointer(desc), C.c_void_p)
+        self.keep = keep
+
+
+class Rows(_Desc):
+    """Device rows [tokens][heads][head_dim] of f32, f16 or bf16 with strides
+    in elements (ditch_cuda_rows)."""
+
+    def __init__(self, data, dtype, heads, token_stride, head_stride):
+        super().__init__(RowsDesc(_dev(data), DTYPE[dtype], heads, token_stride, head_stride), data)
+
+    @classmethod
+    def of(cls, t):
+        """The rows of a [tokens, heads, head_dim] tensor whose last dimension is contiguous."""
+        name = {"float32": "f32", "float16": "f16", "bfloat16": "bf16"}.get(str(t.dtype).replace("torch.", ""))
+        if name is None or t.dim() != 3 or t.stride(2) != 1:
+            raise ValueError("rows are [tokens, heads, head_dim] of f32, f16 or bf16, contiguous in the last dimension")
+        return cls(t, name, t.shape[1], t.stride(0), t.stride(1))
+
+
+class Rope(_Desc):
+    """Device cos / sin tables [table_len][half] f32 (ditch_cuda_rope); style 0 = neox, 1 = gptj."""
+
+    def __init__(self, cos_t, sin_t, table_len, half, style=0):
+        super().__init__(RopeDesc(_dev(cos_t), _dev(sin_t), table_len, half, style), cos_t, sin_t)
+
+
+class KvBatch(_Desc):
+    """The sequences of a call over a paged cache (ditch_cuda_kv_batch):
+    device int32 offsets [n_seqs + 1], lens [n_seqs], pages [n_seqs][max_pages]."""
+
+    def __init__(self, offsets, lens, pages, n_seqs, n_tokens, max_new, max_len, max_pages):
+        super().__init__(KvBatchDesc(n_seqs, n_tokens, max_new, max_len, max_pages, _dev(offsets), _dev(lens),
+                                     _dev(pages)), offsets, lens, pages)
+
+
+class Ragged(_Desc):
+    """Ragged sequences of contiguous rows (ditch_cuda_ragged): device int32
+    q_offsets and kv_offsets [n_seqs + 1]."""
+
+    def __init__(self, q_offsets, kv_offsets, n_seqs, n_q, n_kv, max_q, max_kv):
+        super().__init__(RaggedDesc(n_seqs, n_q, n_kv, max_q, max_kv, _dev(q_offsets), _dev(kv_offsets)), q_offsets,
+                         kv_offsets)
+
+
+class KvCache(_Desc):
+    """A pool of pages of one layer's 8-bit keys and values in device memory
+    (ditch_cuda_kv_cache): codes [n_pages][kv_heads][page_tokens][head_dim],
+    f32 scales [n_pages][kv_heads][page_tokens / block_tokens]. The calls are
+    queued on `stream` (a cudaStream_t as an int, 0 the default stream)."""
+
+    FORMATS = {"int8": 0, "fp8": 1}
+
+    def __init__(self, device, format, k, v, k_scale, v_scale, kv_heads, head_dim, page_tokens, block_tokens, n_pages):
+        super().__init__(KvCacheDesc(self.FORMATS[format], kv_heads, head_dim, page_tokens, block_tokens, n_pages,
+                                     _dev(k), _dev(v), _dev(k_scale), _dev(v_scale)), k, v, k_scale, v_scale)
+        self.dev = device
+
+    def append(self, batch, k, v, q=None, q_out=None, rope=None, k_out=None, v_out=None, stream=0):
+        """Rotates the batch's queries (to q_out) and keys and stores keys and
+        values as 8-bit codes (ditch_cuda_kv_append)."""
+        st = lib().ditch_cuda_kv_append(self.dev.h, self.ref, batch.ref, rope and rope.ref, q and q.ref,
+                                        q_out and q_out.ref, k.ref, v.ref, k_out and k_out.ref, v_out and v_out.ref,
+                                        stream)
+        if st:
+            check(st)
+
+    def read(self, batch, k_out, v_out, stream=0):
+        """The batch's tokens back as rows, code * scale (ditch_cuda_kv_read)."""
+        st = lib().ditch_cuda_kv_read(self.dev.h, self.ref, batch.ref, k_out.ref, v_out.ref, stream)
+        if st:
+            check(st)
+
+    def attention_workspace(self, batch, q_heads):
+        """Bytes of (zero-filled) workspace that attention needs for such a batch."""
+        return lib().ditch_cuda_kv_attention_workspace(self.dev.h, self.ref, batch.ref, q_heads)
+
+    def attention(self, batch, q, out, scale, window=0, sinks=0, workspace=None, workspace_bytes=0, stream=0):
+        """Causal attention of the batch's rows over their cached tokens, with
+        a sliding window and sinks (ditch_cuda_kv_attention)."""
+        st = lib().ditch_cuda_kv_attention(self.dev.h, self.ref, batch.ref, q.ref, out.ref, scale, window, sinks,
+                                           _dev(workspace), workspace_bytes, stream)
+        if st:
+            check(st)
 
 
 class Group:

@@ -387,6 +387,118 @@ int ditch_cuda_edit_weight_bf16(ditch_cuda_device *dev, void *w, size_t rows, si
 int ditch_cuda_edit_weight_bf16_noalloc(void *w, size_t rows, size_t cols, const float *r, float alpha,
                                         void *stream);
 
+/* ---- paged 8-bit key / value cache, and attention with a window ----
+ * Operators over device memory for a host that keeps its own cache (the
+ * reference's KvCache, src/model.zig:2586-2724, is one contiguous f32 array).
+ * Every pointer is a device pointer of the device's GPU; the work is queued
+ * on `stream` (a cudaStream_t, NULL for the default stream) and the call
+ * returns without waiting and allocates nothing, so the calls can be captured
+ * in a graph. What the kernels find wrong in device data (an offset, a length
+ * or a page outside its bounds) is left out and sets the device's status
+ * word: the next ditch_cuda_synchronize returns DITCH_CUDA_INVALID. */
+#define DITCH_KV_INT8 0 /* codes -127..127 */
+#define DITCH_KV_FP8 1  /* codes E4M3 (largest 448) */
+
+/* A pool of pages for one layer. A page holds page_tokens consecutive tokens
+ * of one sequence; every block_tokens of them share one scale per kv head:
+ * value = code * scale. head_dim a multiple of 16, at most 128; page_tokens
+ * 16, 32, 64, 128 or 256; block_tokens 16, 32 or 64, at most page_tokens.
+ * Codes 16-byte, scales 4-byte aligned. */
+typedef struct {
+    int format;
+    int kv_heads, head_dim;
+    int page_tokens, block_tokens;
+    size_t n_pages;
+    void *k, *v;              /* [n_pages][kv_heads][page_tokens][head_dim] bytes */
+    float *k_scale, *v_scale; /* [n_pages][kv_heads][page_tokens / block_tokens] */
+} ditch_cuda_kv_cache;
+
+/* The sequences of a call. Sequence b has tokens offsets[b] .. offsets[b + 1]
+ * of the call's rows, the last ones of its lens[b] tokens (row i of it is at
+ * position lens[b] - (offsets[b + 1] - offsets[b]) + i); token t of it lies in
+ * page pages[b * max_pages + t / page_tokens]. Pages outside a window may hold
+ * any number. The host's counts bound the device's: n_tokens rows, max_new
+ * rows and max_len tokens of one sequence. */
+typedef struct {
+    size_t n_seqs, n_tokens, max_new, max_len, max_pages;
+    const int32_t *offsets; /* [n_seqs + 1] */
+    const int32_t *lens;    /* [n_seqs] */
+    const int32_t *pages;   /* [n_seqs][max_pages] */
+} ditch_cuda_kv_batch;
+
+/* Rows [tokens][heads][head_dim] of f32, f16 or bf16 (DITCH_DTYPE_*), with
+ * strides in elements; the dimensions of a head are contiguous. Rows whose
+ * heads are all 16-byte aligned are read and written 16 bytes at a time. */
+typedef struct {
+    void *data;
+    int dtype, heads;
+    size_t token_stride, head_stride;
+} ditch_cuda_rows;
+
+/* Rotation of the first 2 * half dimensions of a head: tables [table_len]
+ * [half] f32, style 0 = neox (rotate half), 1 = gptj (interleaved), as
+ * ditch_cuda_rope_rows; half a multiple of 8. */
+typedef struct {
+    const float *cos_t, *sin_t;
+    size_t table_len, half;
+    int style;
+} ditch_cuda_rope;
+
+/* Appends keys and values to the cache: the batch's rows of k are rotated
+ * (rope NULL: not), rounded to codes and stored with those of v. A block's
+ * scale is the largest magnitude stored in it / 127 or 448 (0 when that is
+ * below 2^-126), codes are round-to-nearest-even of x * (1 / scale). A block
+ * whose first token is new starts afresh; one that holds earlier tokens keeps
+ * at least its scale, and when that grows the earlier codes are rounded
+ * again to the new one. An infinity or NaN makes its block's scale NaN. q
+ * (with q_out) is rotated to q_out; k_out and v_out, when given, get the rows
+ * that were stored, rotated and not rounded to codes. q_out may be q. The
+ * rows q, k and v share one dtype. Pages being written belong to one
+ * sequence. */
+int ditch_cuda_kv_append(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache, const ditch_cuda_kv_batch *batch,
+                         const ditch_cuda_rope *rope, const ditch_cuda_rows *q, const ditch_cuda_rows *q_out,
+                         const ditch_cuda_rows *k, const ditch_cuda_rows *v, const ditch_cuda_rows *k_out,
+                         const ditch_cuda_rows *v_out, void *stream);
+/* The batch's tokens back as rows: code * scale, rounded once to the rows'
+ * dtype. */
+int ditch_cuda_kv_read(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache, const ditch_cuda_kv_batch *batch,
+                       const ditch_cuda_rows *k_out, const ditch_cuda_rows *v_out, void *stream);
+/* Attention of the batch's rows over their sequences' cached tokens (their
+ * own included: append first). The row at position p sees token j when
+ * j <= p and (window is 0, or j > p - window, or j < sinks):
+ * out = sum softmax(scale * q . k) v, zero for a row that sees nothing. Query
+ * head h reads kv head h / (heads / kv_heads). What a row does not see does
+ * not change it, whatever its codes; a scale that is not finite makes
+ * the rows that see its block not finite. f32 out is computed to f32
+ * rounding, f16 and bf16 out with the softmax weights rounded to f16. The
+ * workspace holds the partial sums of sequences split over the GPU: at least
+ * ditch_cuda_kv_attention_workspace bytes for the same cache, batch sizes and
+ * query heads (0: none is needed), 16-byte aligned, zero-filled before its
+ * first use and then left to these calls, one at a time; it may serve batches
+ * of other sizes that fit. */
+size_t ditch_cuda_kv_attention_workspace(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache,
+                                         const ditch_cuda_kv_batch *batch, size_t q_heads);
+int ditch_cuda_kv_attention(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache, const ditch_cuda_kv_batch *batch,
+                            const ditch_cuda_rows *q, const ditch_cuda_rows *out, float scale, size_t window,
+                            size_t sinks, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Ragged sequences of contiguous rows: sequence b has query rows q_offsets[b]
+ * .. q_offsets[b + 1] (the last of its tokens) and key / value rows
+ * kv_offsets[b] .. kv_offsets[b + 1] (all of them). */
+typedef struct {
+    size_t n_seqs, n_q, n_kv, max_q, max_kv;
+    const int32_t *q_offsets, *kv_offsets; /* [n_seqs + 1] */
+} ditch_cuda_ragged;
+
+/* The same attention over contiguous f16 or bf16 rows (q, k, v and out of one
+ * dtype; head_dim a multiple of 8, at most 128): a prompt's own queries, keys
+ * and values. A row that sees a key or value that is not finite gets what the
+ * formula gives; one that does not see it is not changed by it. The softmax
+ * weights are rounded to the rows' dtype for the products with the values. */
+int ditch_cuda_window_attention(ditch_cuda_device *dev, const ditch_cuda_ragged *seqs, size_t head_dim,
+                                const ditch_cuda_rows *q, const ditch_cuda_rows *k, const ditch_cuda_rows *v,
+                                const ditch_cuda_rows *out, float scale, size_t window, size_t sinks, void *stream);
+
 /* ---- one resident weight and its dequant-fused GEMM ----
  * The product behind `matmulT` (src/tensor.zig:1023-1045) for one weight
  * kept in HBM in its stored format: FP8 blocks, MXFP4 and INT4 groups of 64k
