@@ -1,6 +1,6 @@
 // Appending keys and values to the paged 8-bit cache, with the rotation of
 // queries and keys on the way, and reading tokens back as rows.
-#include "kvcache.cuh"
+#include "kv_range.cuh"
 
 namespace ditch {
 namespace kv {
@@ -131,8 +131,9 @@ __device__ __forceinline__ uint2 encode8(bool fp8, const float (&x)[8], float f)
 
 __device__ __forceinline__ void decode4(bool fp8, uint32_t u, float *x) {
     if (fp8) {
-        const float2 a = e4m3x2_f32(u & 0xffff), b = e4m3x2_f32(u >> 16);
-        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+        uint32_t even = e4m3_pair_f16(u << 8), odd = e4m3_pair_f16(u);
+        const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&even)), b = __half22float2(*reinterpret_cast<__half2 *>(&odd));
+        x[0] = a.x * 256.0f, x[1] = b.x * 256.0f, x[2] = a.y * 256.0f, x[3] = b.y * 256.0f;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] = static_cast<float>(static_cast<int8_t>(u >> (8 * i)));

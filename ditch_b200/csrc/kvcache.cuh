@@ -139,13 +139,5 @@ __device__ __forceinline__ void store1(const Rows &r, long long at, float v) {
     else static_cast<__half *>(r.p)[at] = __float2half_rn(v);
 }
 
-// ---- codes ------------------------------------------------------------------------
-__device__ __forceinline__ float e4m3_value(uint32_t code) { return e4m3x2_f32(code).x; }
-
-// One code's value without its scale.
-__device__ __forceinline__ float code_value(bool fp8, uint32_t code) {
-    return fp8 ? e4m3_value(code & 0xff) : static_cast<float>(static_cast<int8_t>(code));
-}
-
 }  // namespace kv
 }  // namespace ditch

@@ -1,5 +1,4 @@
-// Attention over the paged 8-bit cache and over contiguous rows: one warp per
-// (row, query head), keys one by one with a running maximum and sum.
+// Attention over contiguous rows: one warp per (row, query head), keys one by one with a running maximum and sum.
 #include "attn_common.cuh"
 #include "kvcache.cuh"
 
@@ -36,40 +35,6 @@ __device__ __forceinline__ int first_key(int p, int window, int sinks) {
     return window && sinks == 0 && p >= window ? p - window + 1 : 0;
 }
 
-__global__ void __launch_bounds__(kRowWarps * 32) k_attend_rows(AttendParams p) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = 4 * lane;
-    const long long row = static_cast<long long>(blockIdx.x) * kRowWarps + warp;
-    if (row >= static_cast<long long>(p.b.n_tokens) * p.q.heads) return;
-    const int tok = static_cast<int>(row / p.q.heads), head = static_cast<int>(row % p.q.heads);
-    int seq = 0;
-    while (seq + 1 < p.b.n_seqs && __ldg(p.b.offsets + seq + 1) <= tok) seq++;
-    const Span a = span_of(p.b, p.c.page_shift, seq, p.status);
-    const int i = tok - a.row0;
-    if (i < 0 || i >= a.n) return;
-    const int pos = a.len - a.n + i, kvh = head / (p.q.heads / p.c.heads);
-    float q[4] = {0, 0, 0, 0};
-    for (int e = 0; e < 4; e++)
-        if (d + e < p.c.dim) q[e] = load1(p.q, tok * p.q.ts + head * p.q.hs + d + e);
-    RowState st;
-    for (int j = first_key(pos, p.window, p.sinks); j <= pos; j = next_key(j, pos, p.window, p.sinks)) {
-        const int page = page_of(p.c, p.b, seq, j, p.status);
-        if (page < 0) continue;
-        float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-        if (d < p.c.dim) {
-            const long long at = code_at(p.c, page, kvh, j) + d, sa = scale_at(p.c, page, kvh, j);
-            const uint32_t uk = *reinterpret_cast<const uint32_t *>(p.c.k + at), uv = *reinterpret_cast<const uint32_t *>(p.c.v + at);
-            for (int e = 0; e < 4; e++) {
-                k[e] = code_value(p.c.fp8, uk >> (8 * e)) * p.c.ks[sa];
-                v[e] = code_value(p.c.fp8, uv >> (8 * e)) * p.c.vs[sa];
-            }
-        }
-        st.key(q, k, v, p.scale * kLog2e);
-    }
-    for (int e = 0; e < 4; e++)
-        if (d + e < p.c.dim)
-            store1(p.out, tok * p.out.ts + head * p.out.hs + d + e, st.m == -INFINITY ? 0.0f : st.o[e] / st.sum);
-}
-
 __global__ void __launch_bounds__(kRowWarps * 32) k_window_rows(WindowParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = 4 * lane;
     const long long row = static_cast<long long>(blockIdx.x) * kRowWarps + warp;
@@ -102,14 +67,6 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_window_rows(WindowParams p) 
 }
 
 }  // namespace
-
-size_t attend_workspace(const Cache &, const Batch &, int, int) { return 0; }
-
-cudaError_t attend(const AttendParams &p, int, cudaStream_t s) {
-    const long long rows = (long long)p.b.n_tokens * p.q.heads;
-    k_attend_rows<<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
-    return cudaGetLastError();
-}
 
 cudaError_t window_attention(const WindowParams &p, int, cudaStream_t s) {
     const long long rows = (long long)p.b.n_q * p.q.heads;

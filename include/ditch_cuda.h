@@ -397,7 +397,7 @@ int ditch_cuda_edit_weight_bf16_noalloc(void *w, size_t rows, size_t cols, const
  * or a page outside its bounds) is left out and sets the device's status
  * word: the next ditch_cuda_synchronize returns DITCH_CUDA_INVALID. */
 #define DITCH_KV_INT8 0 /* codes -127..127 */
-#define DITCH_KV_FP8 1  /* codes E4M3 (largest 448) */
+#define DITCH_KV_FP8 1  /* codes E4M3 (largest 448; the NaN codes are never stored and read as +-480) */
 
 /* A pool of pages for one layer. A page holds page_tokens consecutive tokens
  * of one sequence; every block_tokens of them share one scale per kv head:
