@@ -1191,6 +1191,14 @@ bool gemm_map_bf16(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t ro
                     CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+bool tensor_map(CUtensorMap *map, CUtensorMapDataType type, int rank, const void *ptr, const cuuint64_t *dims,
+                const cuuint64_t *strides, const cuuint32_t *box, CUtensorMapSwizzle swizzle) {
+    EncodeTiledFn fn = encode_fn();
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    return fn && fn(map, type, rank, const_cast<void *>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 size_t skinny_split_bytes(int rows, int splits) { return (size_t)((rows + 15) / 16) * splits * 256 * sizeof(float); }
 
 size_t gemm_stream_k_bytes(int grid, int bn, bool dual) {

@@ -119,6 +119,11 @@ cudaError_t launch_gemm_pair(const GemmOperand &a, const GemmOperand *a2, const 
 bool gemm_map_bf16(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows, uint64_t row_bytes,
                    uint32_t box_rows);
 
+// A tiled tensor map of `rank` dimensions (strides in bytes, from the second
+// dimension on), zeros out of bounds.
+bool tensor_map(CUtensorMap *map, CUtensorMapDataType type, int rank, const void *ptr, const cuuint64_t *dims,
+                const cuuint64_t *strides, const cuuint32_t *box, CUtensorMapSwizzle swizzle);
+
 cudaError_t launch_gemm(int fmt, const GemmOperand &a, const GemmOperand *a2, const GemmOperand &b,
                         GemmParams p, int num_sms, cudaStream_t stream);
 

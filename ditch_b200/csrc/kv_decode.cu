@@ -12,10 +12,11 @@
 // with the block's scales applied to the f32 products: s = sk c_r S^T where
 // c_r holds the softmax scale and the power of two by which row r of Q was
 // brought into f16's range, and sv as the block's P . V is added to the f32
-// sums. Codes go from global memory to registers in 16-byte pieces and from
-// there to MMA operands without shared memory: the order of the reduction is
-// free, so a lane's 32 (of K) or 16 (of V) contiguous dimensions are the
-// ones its fragments name.
+// sums. Each warp keeps a ring of blocks of its own in shared memory, filled
+// by TMA three blocks ahead (a box of 16 tokens, rows padded with zeros to 64
+// or 128 bytes, swizzled so that the reads below meet no bank twice), and
+// waits for nobody else. The order of the reduction is free, so a lane's 32
+// (of K) or 16 (of V) contiguous dimensions are the ones its fragments name.
 //
 // Online softmax per warp in base 2. The reference maximum moves only when a
 // score passes it by kLazy: weights stay below 2^kLazy, well inside f16, and
@@ -23,11 +24,15 @@
 //
 // f32 rows: Q and P are each split into two f16 (22 bits), two MMAs for one.
 //
-// A sequence's blocks are split over CTAs when there are few rows; partial
-// sums (f32) go to the workspace and the CTA that arrives last adds them in
-// order, so results do not depend on timing.
+// The blocks of all work items (sequence, key / value head, row tile), one
+// item after another, are divided evenly over as many CTAs as the GPU holds,
+// whatever the sequences' lengths. A CTA's share may begin and end inside an
+// item: it leaves that item's sums (f32) in the workspace, and the CTA that
+// brings an item's last part adds the parts in order, so results do not
+// depend on timing.
 #include <algorithm>
 
+#include "gemm.cuh"
 #include "kv_range.cuh"
 
 namespace ditch {
@@ -38,7 +43,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kBlk = 16;         // tokens of one step of a warp
 constexpr float kLazy = 8.0f;
-constexpr int kCounters = 16384;  // split work items: their arrival counters, first in the workspace
+constexpr int kCounters = 4096;  // arrival counters (one per CTA), first in the workspace
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -66,468 +71,623 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-struct Plan {
-    int nt;             // tiles of 8 rows per CTA
-    int row_tiles;      // CTAs over the rows of a (sequence, kv head)
-    int splits, len;    // CTAs over its blocks at most, and the blocks of one
-    long long items;
-};
+// A warp's ring: kDepth blocks of K and V codes, rows of DP bytes swizzled by
+// TMA (16-byte chunk c of row r lies at c ^ (r & 7) for 128-byte rows, at
+// c ^ (r / 2 & 3) for 64-byte rows).
+constexpr int kDepth = 3;
 
-template <int DP, int NT, bool SPLIT, bool FP8>
-struct Step {
-    static constexpr int kK = DP / 64;  // 16-byte pieces of a key per lane
-    uint4 k[2][kK];                     // tokens g and g + 8, dimensions (DP / 4) t ...
-    uint32_t v[4][DP / 32];             // tokens 2t, 2t + 1, 2t + 8, 2t + 9, dimensions (DP / 8) g ...
-    float sk, sv;
-    int tok;                            // first token, or -1: nothing to see
-};
+template <int DP>
+__device__ __forceinline__ const uint8_t *chunk_of(const uint8_t *tile, int r, int c) {
+    return tile + r * DP + ((DP == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
+}
 
-// The codes and scales of block `blk` of the range (a page of 16 tokens or
-// more holds whole blocks).
-template <int DP, int NT, bool SPLIT, bool FP8>
-__device__ __forceinline__ void load_step(Step<DP, NT, SPLIT, FP8> &s, const Cache &c, int head, int tok, int page, int lane) {
-    using St = Step<DP, NT, SPLIT, FP8>;
-    s.tok = page < 0 ? -1 : tok;
-    if (page < 0) return;
-    const int g = lane >> 2, t = lane & 3;
-    const long long at = code_at(c, page, head, tok), sa = scale_at(c, page, head, tok);
-    const uint8_t *kp = c.k + at + (long long)g * c.dim + t * (DP / 4);
-    const uint8_t *vp = c.v + at + (long long)(2 * t) * c.dim + g * (DP / 8);
-#pragma unroll
-    for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int i = 0; i < St::kK; i++) {
-            const bool in = t * (DP / 4) + 16 * i < c.dim;
-            s.k[r][i] = in ? __ldcs(reinterpret_cast<const uint4 *>(kp + (long long)(8 * r) * c.dim + 16 * i)) : make_uint4(0, 0, 0, 0);
-        }
-    const bool in = g * (DP / 8) < c.dim;
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const uint8_t *row = vp + (long long)((r & 1) + 8 * (r >> 1)) * c.dim;
-        if (DP == 128) {
-            const uint4 u = in ? __ldcs(reinterpret_cast<const uint4 *>(row)) : make_uint4(0, 0, 0, 0);
-            s.v[r][0] = u.x, s.v[r][1] = u.y, s.v[r][DP / 32 - 2] = u.z, s.v[r][DP / 32 - 1] = u.w;
-        } else {
-            const uint2 u = in ? __ldcs(reinterpret_cast<const uint2 *>(row)) : make_uint2(0, 0);
-            s.v[r][0] = u.x, s.v[r][1] = u.y;
-        }
-    }
-    s.sk = __ldg(c.ks + sa);
-    s.sv = __ldg(c.vs + sa);
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap *map, uint64_t *bar, void *dst, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(y), "r"(z)
+        : "memory");
+}
+
+// d += a * b on two f32 each.
+__device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, float b0, float b1) {
+    uint64_t a, b, d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(b0), "f"(b1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(d0), "f"(d1));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
 }
 
 struct Smem {
-    float m[kWarps][32], l[kWarps][32];
-    int last;
+    uint64_t full[kWarps][kDepth];
+    float m[kWarps][32], l[kWarps][32], k[kWarps][32];
+    long long sums[kWarps], at;
+    int seq, last, abort;
 };
 
+// CTAs of four warps to an SM, by their registers.
+template <int NT, bool SPLIT>
+constexpr int ctas_per_sm() {
+    return NT == 1 ? (SPLIT ? 3 : 4) : 2;
+}
+
+// Shared memory from a 1024-byte aligned base: the rings, over which the
+// warps' sums go at the end of an item, and Q.
+template <int DP, int NT, bool SPLIT>
+struct Layout {
+    static constexpr int kTile = kBlk * DP;  // bytes of a block's K or V
+    static constexpr int kRing = kWarps * kDepth * 2 * kTile;
+    static constexpr int kO = kWarps * 8 * NT * DP * 4;
+    static constexpr int kQ = (SPLIT ? 2 : 1) * 8 * NT * (DP + 8) * 2;
+    static constexpr int kQAt = kRing > kO ? kRing : kO;
+    static constexpr int kBytes = 1024 + kQAt + kQ;
+};
+
+// A sequence's work: row tiles per head, and block slots of each (an upper
+// bound where there are several tiles; slots past a tile's blocks are empty).
+struct Work {
+    Span a;
+    int tiles, slots;
+};
+
+template <int ROWS>
+__device__ __forceinline__ Work work_of(const AttendParams &p, int group, int seq) {
+    Work w;
+    w.a = span_of(p.b, p.c.page_shift, seq, p.status);
+    w.tiles = (w.a.n * group + ROWS - 1) / ROWS;
+    w.slots = 0;
+    if (w.tiles == 1) {
+        w.slots = range_of(w.a.len - w.a.n, w.a.len - 1, p.window, p.sinks, kBlk).n;
+    } else if (w.tiles > 1) {
+        const long long all = (w.a.len - 1) / kBlk + 1;
+        const long long some = (p.sinks + kBlk - 1) / kBlk + (static_cast<long long>(p.window) + ROWS / group + 1) / kBlk + 2;
+        w.slots = static_cast<int>(p.window && some < all ? some : all);
+    }
+    return w;
+}
+
 template <int DP, int NT, bool SPLIT, bool FP8>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) k_attend(AttendParams p, Plan plan) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
+    k_attend(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, AttendParams p) {
+    using L = Layout<DP, NT, SPLIT>;
     constexpr int kRows = 8 * NT;
     constexpr int kQs = DP + 8;        // row stride of Q in shared memory (f16)
     constexpr int kSteps = DP / 16;    // MMA steps over the dimensions
     constexpr int kMt = DP / 16;       // tiles of 16 dimensions of O^T
-    constexpr float kUnit = FP8 ? 256.0f : 1.0f;  // value of a code in f16
+    constexpr bool kBiased = !FP8 && !SPLIT;  // V codes + 1152: see below
+    constexpr int kPart = kRows * (DP + 2);   // floats of a part: sums, maxima, sums of weights
+    extern __shared__ uint8_t smem_raw[];
     __shared__ Smem sm;
-    __shared__ __align__(16) __half s_q[(SPLIT ? 2 : 1) * kRows * kQs];
-    __shared__ __align__(16) float s_o[kRows * DP];
     __shared__ float s_c[kRows];
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __half *s_q = reinterpret_cast<__half *>(base + L::kQAt);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x;
-    int item = blockIdx.y + gridDim.y * blockIdx.z;  // (sequence, kv head, row tile)
-    if (item >= plan.items) return;
-    const int tile = item % plan.row_tiles, head = item / plan.row_tiles % p.c.heads, seq = item / plan.row_tiles / p.c.heads;
-    const Span a = span_of(p.b, p.c.page_shift, seq, p.status);
-    const int group = p.q.heads / p.c.heads, rows = a.n * group, r0 = tile * kRows;
-    if (r0 >= rows) return;
-    const int n_rows = min(kRows, rows - r0), first = a.len - a.n;
-    const int p_lo = first + r0 / group, p_hi = first + (r0 + n_rows - 1) / group;
-    const Range range = range_of(p_lo, p_hi, p.window, p.sinks, kBlk);
-    const int per = max(plan.len, (range.n + plan.splits - 1) / plan.splits);
-    const int my_splits = (range.n + per - 1) / per;
-    if (split >= my_splits) return;
-    const int b_lo = split * per, b_hi = min(range.n, b_lo + per);
+    const int group = p.q.heads / p.c.heads;
+    uint8_t *ring = base + warp * (kDepth * 2 * L::kTile);
+    uint64_t *full = sm.full[warp];
+    if (lane == 0) {
+        for (int i = 0; i < kDepth; i++) mbar_init(&full[i], 1);
+        fence_barrier_init();
+    }
+    if (tid == 0) sm.abort = 0;
 
-    // this warp's blocks are b_lo + warp, + kWarps, ...; lane i looks up the page of the i-th
-    int b = b_lo + warp, ahead = 0;
-    int pages = -1;
-    auto look_up = [&]() {
-        const int x = b_lo + warp + kWarps * (ahead + lane);
-        pages = x < b_hi ? page_of(p.c, p.b, seq, range.token(x, kBlk), p.status) : -1;
-    };
-    look_up();
-
-    // ---- Q to f16, each row by a power of two to below 2 ----
-    for (int r = warp; r < kRows; r += kWarps) {
-        float x[DP / 32];
-        uint32_t top = 0;
-        const int row = r0 + r, i = row / group;
-        const long long at = (a.row0 + i) * p.q.ts + (head * group + row - i * group) * p.q.hs;
+    // ---- this CTA's share of the block slots: [pos, end) ----
+    const int chunk = (p.b.n_seqs + kThreads - 1) / kThreads;  // sequences a thread counts
+    const int c_lo = min(tid * chunk, p.b.n_seqs), c_hi = min(c_lo + chunk, p.b.n_seqs);
+    long long mine = 0;
+    for (int x = c_lo; x < c_hi; x++) {
+        const Work w = work_of<kRows>(p, group, x);
+        mine += static_cast<long long>(w.tiles) * w.slots * p.c.heads;
+    }
+    long long upto = mine;
 #pragma unroll
-        for (int e = 0; e < DP / 32; e++) {
-            const int d = lane + 32 * e;
-            x[e] = r < n_rows && d < p.c.dim ? load1(p.q, at + d) : 0.0f;
-            top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        int e2 = static_cast<int>(top >> 23) - 127;
-        e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
-        if (lane == 0) s_c[r] = p.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23) * kUnit;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 31) sm.sums[warp] = upto;
+    __syncthreads();
+    long long total = 0;
 #pragma unroll
-        for (int e = 0; e < DP / 32; e++) {
-            // pairs of codes are taken as (0, 2) and (1, 3) of four
-            int d = lane + 32 * e;
-            d = FP8 && ((d & 3) == 1 || (d & 3) == 2) ? d ^ 3 : d;
-            const float y = x[e] * down;
-            const __half h = __float2half_rn(y);
-            s_q[r * kQs + d] = h;
-            if (SPLIT) s_q[(kRows + r) * kQs + d] = __float2half_rn(y - __half2float(h));
+    for (int w = 0; w < kWarps; w++) {
+        if (w < warp) upto += sm.sums[w];
+        total += sm.sums[w];
+    }
+    const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kWarps));
+    long long pos = per * blockIdx.x;
+    const long long end = min(total, pos + per);
+    if (pos >= end) return;
+    if (upto - mine <= pos && pos < upto) {
+        long long at = upto - mine;
+        int x = c_lo;
+        for (;; x++) {
+            const Work w = work_of<kRows>(p, group, x);
+            const long long n = static_cast<long long>(w.tiles) * w.slots * p.c.heads;
+            if (pos < at + n) break;
+            at += n;
         }
+        sm.seq = x;
+        sm.at = at;
     }
     __syncthreads();
+    int seq = sm.seq;
+    Work work = work_of<kRows>(p, group, seq);
+    int item = static_cast<int>((pos - sm.at) / work.slots);  // of the sequence: head * tiles + tile
+    int off = static_cast<int>(pos - sm.at - static_cast<long long>(item) * work.slots);
 
-    float c_row[NT][2];
-    int top_key[NT][2], low_key[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int r = 8 * n + 2 * t + e;
-            c_row[n][e] = s_c[r];
-            top_key[n][e] = r < n_rows ? first + (r0 + r) / group : -1;
-            low_key[n][e] = p.window ? top_key[n][e] - p.window + 1 : 0;
-        }
-    uint32_t qf[NT == 1 && !SPLIT ? kSteps : 1][2];
-    if (NT == 1 && !SPLIT) {
-#pragma unroll
-        for (int s = 0; s < kSteps; s++) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(s_q + g * kQs + t * (DP / 4) + 4 * s);
-            qf[NT == 1 && !SPLIT ? s : 0][0] = u.x;
-            qf[NT == 1 && !SPLIT ? s : 0][1] = u.y;
-        }
-    }
+    const int page_mask = (1 << p.c.page_shift) - 1;
+    uint32_t phase = 0;  // bit st: parity of the next completion of stage st
+    int st = 0;          // the ring's next stage
+    bool dead = false;   // a wait ran out
 
-    float o[NT][kMt][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-#pragma unroll
-        for (int j = 0; j < kMt; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[n][j][e] = 0.0f;
-        m[n][0] = m[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.0f;
-    }
+    while (pos < end) {
+        const Span a = work.a;
+        const int n_slots = static_cast<int>(min(static_cast<long long>(work.slots - off), end - pos));
+        const int head = item / work.tiles, tile = item - head * work.tiles;
+        const int rows = a.n * group, r0 = tile * kRows, n_rows = min(kRows, rows - r0), first = a.len - a.n;
+        const int p_lo = first + r0 / group, p_hi = first + (r0 + n_rows - 1) / group;
+        const Range range = range_of(p_lo, p_hi, p.window, p.sinks, kBlk);
+        const int b_lo = off, b_hi = min(range.n, off + n_slots);
 
-    // The page lookups and loads of a step come one step ahead of its use.
-    auto fetch = [&](Step<DP, NT, SPLIT, FP8> &s, int i) {
-        const int x = b_lo + warp + kWarps * i;
-        if (i - ahead >= 32) {
-            ahead += 32;
-            look_up();
-        }
-        const int page = __shfl_sync(0xffffffffu, pages, i - ahead);
-        if (x < b_hi) load_step<DP, NT, SPLIT, FP8>(s, p.c, head, range.token(x, kBlk), page, lane);
-        else s.tok = -1;
-    };
+        // ---- this warp's blocks: b_lo + warp, + kWarps, ...; lane i looks up the page of the i-th ----
+        int ahead = 0, pages = -1;
+        auto look_up = [&]() {
+            const int x = b_lo + warp + kWarps * (ahead + lane);
+            pages = x < b_hi ? page_of(p.c, p.b, seq, range.token(x, kBlk), p.status) : -1;
+        };
+        look_up();
+        // a block under way: its first token (-1: nothing to see) and scales
+        struct Under {
+            int tok;
+            float sk, sv;
+        };
+        auto fetch = [&](int stage, int i) {
+            Under u;
+            u.tok = -1;
+            u.sk = u.sv = 0.0f;
+            if (i - ahead >= 32) {
+                ahead += 32;
+                look_up();
+            }
+            const int page = __shfl_sync(0xffffffffu, pages, i - ahead);
+            if (page < 0) return u;
+            u.tok = range.token(b_lo + warp + kWarps * i, kBlk);
+            if (lane == 0) {
+                uint8_t *tile_at = ring + stage * 2 * L::kTile;
+                const int y = (head << p.c.page_shift) + (u.tok & page_mask);
+                mbar_arrive_expect_tx(&full[stage], 2 * L::kTile);
+                tma_load_3d(&k_map, &full[stage], tile_at, y, page);
+                tma_load_3d(&v_map, &full[stage], tile_at + L::kTile, y, page);
+            }
+            const long long sa = scale_at(p.c, page, head, u.tok);
+            u.sk = __ldg(p.c.ks + sa);
+            u.sv = __ldg(p.c.vs + sa);
+            return u;
+        };
+        auto next = [](int s) { return s + 1 == kDepth ? 0 : s + 1; };
 
-    auto use = [&](const Step<DP, NT, SPLIT, FP8> &s) {
-        if (s.tok < 0) return;
-        // ---- S^T = K . Q^T ----
-        float sc[NT][4];
+        // ---- Q rows into registers, the first blocks under way, Q to f16 ----
+        float qx[kRows / kWarps][DP / 32];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int i = 0; i < kRows / kWarps; i++) {
+            const int r = warp + kWarps * i, row = r0 + r, tok = row / group;
+            const long long at = (a.row0 + tok) * p.q.ts + (head * group + row - tok * group) * p.q.hs;
 #pragma unroll
-            for (int e = 0; e < 4; e++) sc[n][e] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < Step<DP, NT, SPLIT, FP8>::kK; i++) {
-            const uint32_t w0[4] = {s.k[0][i].x, s.k[0][i].y, s.k[0][i].z, s.k[0][i].w};
-            const uint32_t w1[4] = {s.k[1][i].x, s.k[1][i].y, s.k[1][i].z, s.k[1][i].w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t f[4];
-                key_pairs<FP8>(w0[j], f[0], f[2]);
-                key_pairs<FP8>(w1[j], f[1], f[3]);
-                const int step = 4 * i + j;
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    if (NT == 1 && !SPLIT) {
-                        mma_f16(sc[n], f, qf[NT == 1 && !SPLIT ? step : 0][0], qf[NT == 1 && !SPLIT ? step : 0][1]);
-                    } else {
-                        const __half *at = s_q + (8 * n + g) * kQs + t * (DP / 4) + 4 * step;
-                        const uint2 u = *reinterpret_cast<const uint2 *>(at);
-                        mma_f16(sc[n], f, u.x, u.y);
-                        if (SPLIT) {
-                            const uint2 w = *reinterpret_cast<const uint2 *>(at + kRows * kQs);
-                            mma_f16(sc[n], f, w.x, w.y);
-                        }
-                    }
-                }
+            for (int e = 0; e < DP / 32; e++) {
+                const int d = lane + 32 * e;
+                qx[i][e] = r < n_rows && d < p.c.dim ? load1(p.q, at + d) : 0.0f;
             }
         }
-        // ---- softmax ----
-        const bool whole = s.tok + kBlk - 1 <= p_lo && (!p.window || s.tok > p_hi - p.window);
-        bool sees[NT][2];
-        bool over = false;
+        Under u0 = fetch(st, 0), u1 = fetch(next(st), 1), u2 = fetch(next(next(st)), 2);
+#pragma unroll
+        for (int i = 0; i < kRows / kWarps; i++) {  // each row by a power of two to below 2
+            const int r = warp + kWarps * i;
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < DP / 32; e++) top = max(top, __float_as_uint(qx[i][e]) & 0x7fffffffu);
+            top = __reduce_max_sync(0xffffffffu, top);
+            int e2 = static_cast<int>(top >> 23) - 127;
+            e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
+            if (lane == 0) s_c[r] = p.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+#pragma unroll
+            for (int e = 0; e < DP / 32; e++) {
+                const int d = lane + 32 * e;
+                const float y = qx[i][e] * down;
+                const __half h = __float2half_rn(y);
+                s_q[r * kQs + d] = h;
+                if (SPLIT) s_q[(kRows + r) * kQs + d] = __float2half_rn(y - __half2float(h));
+            }
+        }
+        __syncthreads();
+
+        float c_row[NT][2];
+        int top_key[NT][2], low_key[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float f = s.sk * c_row[n][e];
-                sc[n][e] *= f;
-                sc[n][e + 2] *= f;
-                sees[n][e] = true;
-                if (!whole) {
-                    const int hi = top_key[n][e], lo = low_key[n][e];
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int key = s.tok + g + 8 * h;
-                        if (key > hi || (key < lo && key >= p.sinks)) sc[n][e + 2 * h] = -INFINITY;
-                    }
-                    sees[n][e] = s.tok <= hi && (s.tok + kBlk > lo || s.tok < p.sinks);
-                }
-                over |= fmaxf(sc[n][e], sc[n][e + 2]) > m[n][e] + kLazy;
+                const int r = 8 * n + 2 * t + e;
+                c_row[n][e] = s_c[r];
+                top_key[n][e] = r < n_rows ? first + (r0 + r) / group : -1;
+                low_key[n][e] = p.window ? top_key[n][e] - p.window + 1 : 0;
             }
-        if (__any_sync(0xffffffffu, over)) {
+        uint32_t qf[NT == 1 && !SPLIT ? kSteps : 1][2];
+        if (NT == 1 && !SPLIT) {
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                const uint2 u = *reinterpret_cast<const uint2 *>(s_q + g * kQs + t * (DP / 4) + 4 * s);
+                qf[NT == 1 && !SPLIT ? s : 0][0] = u.x;
+                qf[NT == 1 && !SPLIT ? s : 0][1] = u.y;
+            }
+        }
+
+        float o[NT][kMt][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int j = 0; j < kMt; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[n][j][e] = 0.0f;
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.0f;
+        }
+
+        auto use = [&](int stage, const Under &s) {
+            if (s.tok < 0 || dead) return;
+            if (!mbar_wait(&full[stage], (phase >> stage) & 1, &sm.abort, p.status)) {
+                dead = true;
+                return;
+            }
+            phase ^= 1u << stage;
+            const uint8_t *kt = ring + stage * 2 * L::kTile, *vt = kt + L::kTile;
+            // ---- S^T = K . Q^T ----
+            // (even and odd steps apart: two chains of dependent MMAs)
+            float sc[NT][4], odd[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sc[n][e] = odd[n][e] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 64; i++) {
+                const uint4 k0 = *reinterpret_cast<const uint4 *>(chunk_of<DP>(kt, g, t * (DP / 64) + i));
+                const uint4 k1 = *reinterpret_cast<const uint4 *>(chunk_of<DP>(kt, g + 8, t * (DP / 64) + i));
+                const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t f[4];
+                    code_pairs<FP8>(w0[j], f[0], f[2]);
+                    code_pairs<FP8>(w1[j], f[1], f[3]);
+                    const int step = 4 * i + j;
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float(&acc)[4] = step & 1 ? odd[n] : sc[n];
+                        if (NT == 1 && !SPLIT) {
+                            mma_f16(acc, f, qf[NT == 1 && !SPLIT ? step : 0][0], qf[NT == 1 && !SPLIT ? step : 0][1]);
+                        } else {
+                            const __half *at = s_q + (8 * n + g) * kQs + t * (DP / 4) + 4 * step;
+                            const uint2 u = *reinterpret_cast<const uint2 *>(at);
+                            mma_f16(acc, f, u.x, u.y);
+                            if (SPLIT) {
+                                const uint2 w = *reinterpret_cast<const uint2 *>(at + kRows * kQs);
+                                mma_f16(acc, f, w.x, w.y);
+                            }
+                        }
+                    }
+                }
+            }
+            // ---- softmax ----
+            const bool whole = s.tok + kBlk - 1 <= p_lo && (!p.window || s.tok > p_hi - p.window);
+            bool sees[NT][2];
+            bool over = false;
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float x = fmaxf(sc[n][e], sc[n][e + 2]);
+                    const float f = s.sk * c_row[n][e];
+                    sc[n][e] = (sc[n][e] + odd[n][e]) * f;
+                    sc[n][e + 2] = (sc[n][e + 2] + odd[n][e + 2]) * f;
+                    sees[n][e] = true;
+                    if (!whole) {
+                        const int hi = top_key[n][e], lo = low_key[n][e];
 #pragma unroll
-                    for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-                    x = fmaxf(x, m[n][e]);
-                    const float keep = m[n][e] == -INFINITY ? 0.0f : exp2f(m[n][e] - x);
-                    m[n][e] = x;
-                    l[n][e] *= keep;
+                        for (int h = 0; h < 2; h++) {
+                            const int key = s.tok + g + 8 * h;
+                            if (key > hi || (key < lo && key >= p.sinks)) sc[n][e + 2 * h] = -INFINITY;
+                        }
+                        sees[n][e] = s.tok <= hi && (s.tok + kBlk > lo || s.tok < p.sinks);
+                    }
+                    over |= fmaxf(sc[n][e], sc[n][e + 2]) > m[n][e] + kLazy;
+                }
+            if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-                    for (int j = 0; j < kMt; j++) {
-                        o[n][j][e] *= keep;
-                        o[n][j][e + 2] *= keep;
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float x = fmaxf(sc[n][e], sc[n][e + 2]);
+#pragma unroll
+                        for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+                        x = fmaxf(x, m[n][e]);
+                        const float keep = m[n][e] == -INFINITY ? 0.0f : exp2f(m[n][e] - x);
+                        m[n][e] = x;
+                        l[n][e] *= keep;
+#pragma unroll
+                        for (int j = 0; j < kMt; j++) {
+                            o[n][j][e] *= keep;
+                            o[n][j][e + 2] *= keep;
+                        }
+                    }
+            }
+            uint32_t pb[NT][2], pl[SPLIT ? NT : 1][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float ref = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+                    sc[n][e] = exp2_fast(sc[n][e] - ref);
+                    sc[n][e + 2] = exp2_fast(sc[n][e + 2] - ref);
+                    l[n][e] += sc[n][e] + sc[n][e + 2];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t u = half2_bits(sc[n][2 * h], sc[n][2 * h + 1]);
+                    pb[n][h] = transpose8x8(u);
+                    if (SPLIT) {
+                        const float2 f = half2_floats(u);
+                        pl[SPLIT ? n : 0][h] = transpose8x8(half2_bits(sc[n][2 * h] - f.x, sc[n][2 * h + 1] - f.y));
                     }
                 }
-        }
-        uint32_t pb[NT][2], pl[SPLIT ? NT : 1][2];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const float ref = m[n][e] == -INFINITY ? 0.0f : m[n][e];
-                sc[n][e] = SPLIT ? exp2f(sc[n][e] - ref) : exp2_fast(sc[n][e] - ref);
-                sc[n][e + 2] = SPLIT ? exp2f(sc[n][e + 2] - ref) : exp2_fast(sc[n][e + 2] - ref);
-                l[n][e] += sc[n][e] + sc[n][e + 2];
             }
+            // ---- O^T += sv V^T . P^T ----
+            // Biased codes: the sums start at -1152 sum(P), from an MMA with the
+            // same rounded P, so the bias cancels within the block's f32 sum (an
+            // error of 2^-23 of 1152 sum(P), about 1e-5 of a typical block's).
+            float zero[NT][4];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t u = half2_bits(sc[n][2 * h], sc[n][2 * h + 1]);
-                pb[n][h] = transpose8x8(u);
-                if (SPLIT) {
-                    const float2 f = half2_floats(u);
-                    pl[SPLIT ? n : 0][h] = transpose8x8(half2_bits(sc[n][2 * h] - f.x, sc[n][2 * h + 1] - f.y));
-                }
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) zero[n][e] = 0.0f;
+                const uint32_t minus[4] = {0xe480e480u, 0xe480e480u, 0xe480e480u, 0xe480e480u};
+                if (kBiased) mma_f16(zero[n], minus, pb[n][0], pb[n][1]);
             }
-        }
-        // ---- O^T += sv V^T . P^T ----
-        float w[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) w[n][e] = sees[n][e] ? s.sv * kUnit : 0.0f;
-#pragma unroll
-        for (int i = 0; i < DP / 32; i++) {
-#pragma unroll
-            for (int half = 0; half < 2; half++) {  // dimensions (DP / 8) g + 4 i + 2 half, + 1
-                uint32_t f[4];
-                value_pairs<FP8>(s.v[0][i], s.v[1][i], half, f[0], f[1]);
-                value_pairs<FP8>(s.v[2][i], s.v[3][i], half, f[2], f[3]);
-                const int j = 2 * i + half;
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_f16(x, f, pb[n][0], pb[n][1]);
-                    if (SPLIT) mma_f16(x, f, pl[SPLIT ? n : 0][0], pl[SPLIT ? n : 0][1]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[n][j][e] = fmaf(x[e], w[n][e & 1], o[n][j][e]);
-                }
-            }
-        }
-    };
-
-    Step<DP, NT, SPLIT, FP8> s0, s1;
-    const int n_steps = b < b_hi ? (b_hi - b + kWarps - 1) / kWarps : 0;
-    fetch(s0, 0);
-    for (int i = 0; i < n_steps; i += 2) {
-        fetch(s1, i + 1);
-        use(s0);
-        fetch(s0, i + 2);
-        use(s1);
-    }
-
-    // ---- the warps' sums, in order ----
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
-            if (m[n][e] == -INFINITY && l[n][e] != 0.0f) m[n][e] = INFINITY;  // only NaN scores: the row is NaN
-            if (g == 0) {
-                sm.m[warp][8 * n + 2 * t + e] = m[n][e];
-                sm.l[warp][8 * n + 2 * t + e] = l[n][e];
-            }
-        }
-    __syncthreads();
-    float keep[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int r = 8 * n + 2 * t + e;
-            float x = sm.m[0][r];
-#pragma unroll
-            for (int w = 1; w < kWarps; w++) x = fmaxf(x, sm.m[w][r]);
-            keep[n][e] = m[n][e] == -INFINITY ? 0.0f : exp2f(m[n][e] - x);
-        }
-    for (int w = 0; w < kWarps; w++) {
-        if (w == warp) {
+            float w[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int j = 0; j < kMt; j++)
+                for (int e = 0; e < 2; e++) w[n][e] = sees[n][e] ? s.sv : 0.0f;
+            // (an E4M3 NaN in memory past the sequence must not meet a weight of 0)
+            const int seen = whole || !FP8 ? kBlk : p_hi + 1 - s.tok;
+            uint32_t v[4][DP / 32];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9, dimensions (DP / 8) g ...
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float2 *d = reinterpret_cast<float2 *>(s_o + (8 * n + 2 * t + e) * DP + g * (DP / 8) + 2 * j);
-                        const float k = keep[n][e];
-                        float2 v = make_float2(o[n][j][e] * k, o[n][j][e + 2] * k);
-                        if (k == 0.0f) v = make_float2(0.0f, 0.0f);
-                        if (w) {
-                            const float2 u = *d;
-                            v.x += u.x;
-                            v.y += u.y;
-                        }
-                        *d = v;
+            for (int r = 0; r < 4; r++) {
+                const int tok = 2 * t + (r & 1) + 8 * (r >> 1);
+                if (DP == 128) {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(chunk_of<DP>(vt, tok, g));
+                    v[r][0] = u.x, v[r][1] = u.y, v[r][DP / 32 - 2] = u.z, v[r][DP / 32 - 1] = u.w;
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(chunk_of<DP>(vt, tok, g >> 1) + 8 * (g & 1));
+                    v[r][0] = u.x, v[r][1] = u.y;
+                }
+                if (FP8 && tok >= seen) {
+#pragma unroll
+                    for (int i = 0; i < DP / 32; i++) v[r][i] = 0;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 32; i++) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {  // dimensions (DP / 8) g + 4 i + 2 half, + 1
+                    uint32_t f[4];
+                    value_pairs<FP8, kBiased>(v[0][i], v[1][i], half, f[0], f[1]);
+                    value_pairs<FP8, kBiased>(v[2][i], v[3][i], half, f[2], f[3]);
+                    const int j = 2 * i + half;
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float x[4] = {zero[n][0], zero[n][1], zero[n][2], zero[n][3]};
+                        mma_f16(x, f, pb[n][0], pb[n][1]);
+                        if (SPLIT) mma_f16(x, f, pl[SPLIT ? n : 0][0], pl[SPLIT ? n : 0][1]);
+                        fma2(o[n][j][0], o[n][j][1], x[0], x[1], w[n][0], w[n][1]);
+                        fma2(o[n][j][2], o[n][j][3], x[2], x[3], w[n][0], w[n][1]);
                     }
+                }
+            }
+        };
+
+        const int n_steps = b_lo + warp < b_hi ? (b_hi - b_lo - warp + kWarps - 1) / kWarps : 0;
+#pragma unroll 1
+        for (int i = 0; i < n_steps; i++) {
+            use(st, u0);
+            __syncwarp();  // every lane has read the stage
+            u0 = u1;
+            u1 = u2;
+            u2 = fetch(st, i + kDepth);
+            st = next(st);
+        }
+        if (dead) {  // give the loads in flight their time before the memory goes to others
+            for (int x = 0; x < kDepth; x++) mbar_try_wait(&full[x], (phase >> x) & 1);
+        }
+
+        // ---- the warps' sums, in order ----
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+                if (m[n][e] == -INFINITY && l[n][e] != 0.0f) m[n][e] = INFINITY;  // only NaN scores: the row is NaN
+                if (g == 0) {
+                    sm.m[warp][8 * n + 2 * t + e] = m[n][e];
+                    sm.l[warp][8 * n + 2 * t + e] = l[n][e];
+                }
+            }
+        __syncthreads();  // the rings are no longer read: the sums go over them
+        float *s_o = reinterpret_cast<float *>(base) + warp * kRows * DP;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < kMt; j += 2)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    *reinterpret_cast<float4 *>(s_o + (8 * n + 2 * t + e) * DP + g * (DP / 8) + 2 * j) =
+                        make_float4(o[n][j][e], o[n][j][e + 2], o[n][j + 1][e], o[n][j + 1][e + 2]);
+        const bool alone = off == 0 && n_slots == work.slots;
+        const long long item_at = pos - off;
+        const int c0 = static_cast<int>(item_at / per), c1 = static_cast<int>((item_at + work.slots - 1) / per);
+        float *parts = reinterpret_cast<float *>(static_cast<uint8_t *>(p.ws) + kCounters * sizeof(int));
+        float *part = parts + (2 * blockIdx.x + (static_cast<int>(blockIdx.x) == c0 ? 1 : 0)) * static_cast<long long>(kPart);
+        if (tid < kRows) {
+            float mx = sm.m[0][tid], sum = 0.0f;
+#pragma unroll
+            for (int w = 1; w < kWarps; w++) mx = fmaxf(mx, sm.m[w][tid]);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float k = sm.m[w][tid] == -INFINITY ? 0.0f : exp2f(sm.m[w][tid] - mx);
+                sm.k[w][tid] = k;
+                sum += sm.l[w][tid] * k;
+            }
+            if (alone) {
+                const float inv = mx == -INFINITY ? 0.0f : 1.0f / sum;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) sm.k[w][tid] *= inv;
+            } else {
+                part[kRows * DP + tid] = mx;
+                part[kRows * DP + kRows + tid] = sum;
+            }
         }
         __syncthreads();
-    }
+        auto put = [&](int r, int d, float4 v) {
+            const int row = r0 + r, i = row / group;
+            const long long at = (a.row0 + i) * p.out.ts + (head * group + row - i * group) * p.out.hs + d;
+            if (d >= p.c.dim) return;
+            if (p.out.vec) {
+                store4(p.out, at, v);
+            } else {
+                store1(p.out, at, v.x);
+                store1(p.out, at + 1, v.y);
+                store1(p.out, at + 2, v.z);
+                store1(p.out, at + 3, v.w);
+            }
+        };
+        const float *all = reinterpret_cast<const float *>(base);
+        for (int x = 4 * tid; x < n_rows * DP; x += 4 * kThreads) {
+            const int r = x / DP;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float k = sm.k[w][r];
+                const float4 u = *reinterpret_cast<const float4 *>(all + w * kRows * DP + x);
+                if (k != 0.0f) {  // (a warp that saw nothing of the row)
+                    v.x = fmaf(k, u.x, v.x);
+                    v.y = fmaf(k, u.y, v.y);
+                    v.z = fmaf(k, u.z, v.z);
+                    v.w = fmaf(k, u.w, v.w);
+                }
+            }
+            if (alone) put(r, x - r * DP, v);
+            else *reinterpret_cast<float4 *>(part + x) = v;
+        }
+        if (!alone) {
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                int *count = static_cast<int *>(p.ws) + c0;
+                sm.last = atomicAdd(count, 1) == c1 - c0;
+                if (sm.last) *count = 0;
+            }
+            __syncthreads();
+            if (sm.last) {
+                __threadfence();
+                auto part_of = [&](int c) { return parts + (2 * c + (c == c0 ? 1 : 0)) * static_cast<long long>(kPart); };
+                for (int x = 4 * tid; x < n_rows * DP; x += 4 * kThreads) {
+                    const int r = x / DP;
+                    float mx = -INFINITY;
+                    for (int c = c0; c <= c1; c++) mx = fmaxf(mx, __ldcg(part_of(c) + kRows * DP + r));
+                    float sum = 0.0f;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int c = c0; c <= c1; c++) {
+                        const float *q = part_of(c);
+                        const float mc = __ldcg(q + kRows * DP + r);
+                        const float4 u = __ldcg(reinterpret_cast<const float4 *>(q + x));
+                        if (mc == -INFINITY) continue;
+                        const float k = exp2f(mc - mx);
+                        sum = fmaf(k, __ldcg(q + kRows * DP + kRows + r), sum);
+                        v.x = fmaf(k, u.x, v.x);
+                        v.y = fmaf(k, u.y, v.y);
+                        v.z = fmaf(k, u.z, v.z);
+                        v.w = fmaf(k, u.w, v.w);
+                    }
+                    const float inv = mx == -INFINITY ? 0.0f : 1.0f / sum;
+                    put(r, x - r * DP, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                }
+            }
+        }
 
-    auto row_ml = [&](int r, float &mx, float &sum) {
-        mx = sm.m[0][r];
-#pragma unroll
-        for (int w = 1; w < kWarps; w++) mx = fmaxf(mx, sm.m[w][r]);
-        sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) sum += sm.m[w][r] == -INFINITY ? 0.0f : sm.l[w][r] * exp2f(sm.m[w][r] - mx);
-    };
-    auto put = [&](int r, int d, float v) {
-        const int row = r0 + r, i = row / group;
-        store1(p.out, (a.row0 + i) * p.out.ts + (head * group + row - i * group) * p.out.hs + d, v);
-    };
-    if (my_splits == 1) {
-        for (int x = tid; x < n_rows * DP; x += kThreads) {
-            const int r = x / DP, d = x - r * DP;
-            if (d >= p.c.dim) continue;
-            float mx, sum;
-            row_ml(r, mx, sum);
-            put(r, d, mx == -INFINITY ? 0.0f : s_o[r * DP + d] / sum);
+        // ---- on to the next item ----
+        pos += n_slots;
+        off = 0;
+        if (pos < end) {
+            item++;
+            if (item == work.tiles * p.c.heads) {
+                item = 0;
+                do {
+                    seq++;
+                    work = work_of<kRows>(p, group, seq);
+                } while (work.slots == 0);
+            }
+            fence_proxy_async_smem();  // the sums were read and written as plain memory, TMA writes there next
+            __syncthreads();
         }
-        return;
-    }
-    // partial sums of this split: rows of DP sums, then maxima and sums
-    float *ws = reinterpret_cast<float *>(static_cast<uint8_t *>(p.ws) + kCounters * sizeof(int));
-    constexpr int kPart = kRows * (DP + 2);
-    float *part = ws + (static_cast<long long>(item) * plan.splits + split) * kPart;
-    for (int x = tid; x < kRows * DP; x += kThreads) part[x] = s_o[x];
-    if (tid < kRows) {
-        float mx, sum;
-        row_ml(tid, mx, sum);
-        part[kRows * DP + tid] = mx;
-        part[kRows * DP + kRows + tid] = sum;
-    }
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        int *count = static_cast<int *>(p.ws) + item;
-        sm.last = atomicAdd(count, 1) == my_splits - 1;
-        if (sm.last) *count = 0;
-    }
-    __syncthreads();
-    if (!sm.last) return;
-    __threadfence();
-    const float *all = ws + static_cast<long long>(item) * plan.splits * kPart;
-    for (int x = tid; x < n_rows * DP; x += kThreads) {
-        const int r = x / DP, d = x - r * DP;
-        float mx = -INFINITY;
-        for (int s = 0; s < my_splits; s++) mx = fmaxf(mx, __ldcg(all + s * kPart + kRows * DP + r));
-        float sum = 0.0f, v = 0.0f;
-        for (int s = 0; s < my_splits; s++) {
-            const float ms = __ldcg(all + s * kPart + kRows * DP + r);
-            if (ms == -INFINITY) continue;
-            const float k = exp2f(ms - mx);
-            sum = fmaf(k, __ldcg(all + s * kPart + kRows * DP + kRows + r), sum);
-            v = fmaf(k, __ldcg(all + s * kPart + x), v);
-        }
-        if (d < p.c.dim) put(r, d, mx == -INFINITY ? 0.0f : v / sum);
     }
 }
 
-// CTAs of 4 warps, three to an SM (two for more than 8 rows). A sequence is
-// split until there are about kWaves rounds of CTAs, so that ragged lengths
-// leave no SM idle for long, but not below kMinTokens once every SM has
-// work, and not below one block per warp before that.
-constexpr int kWaves = 12, kMinTokens = 512;
-
-Plan plan_of(const Cache &c, const Batch &b, int q_heads, int sms, bool split_f32, int seen) {
-    Plan p;
-    const long long rows = (long long)b.max_new * (q_heads / c.heads);
-    p.nt = rows <= 8 ? 1 : rows <= 16 || split_f32 ? 2 : 4;
-    p.row_tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-    p.items = (long long)b.n_seqs * c.heads * p.row_tiles;
-    const int tokens = seen;
-    const long long want = ((long long)sms * 3 * kWaves + p.items - 1) / p.items;
-    long long len = std::max<long long>((tokens + want - 1) / want, kBlk * kWarps);
-    if (p.items >= sms) len = std::max<long long>(len, kMinTokens);
-    p.len = (int)((len + kBlk - 1) / kBlk);
-    p.splits = p.items > kCounters ? 1 : (tokens + p.len * kBlk - 1) / (p.len * kBlk);
-    return p;
+// Tiles of 8 rows per CTA. More rows than a CTA takes become row tiles that
+// each read the cache.
+int tiles_of(const Cache &c, int max_new, int q_heads, bool split_f32) {
+    const long long rows = (long long)max_new * (q_heads / c.heads);
+    return rows <= 8 ? 1 : rows <= 16 || split_f32 ? 2 : 4;
 }
 
 template <int DP, int NT, bool SPLIT>
-cudaError_t launch2(const AttendParams &p, const Plan &plan, cudaStream_t s) {
-    const long long ny = std::min<long long>(plan.items, 32768), nz = (plan.items + ny - 1) / ny;
-    if (nz > 65535) return cudaErrorInvalidValue;
-    const dim3 grid(plan.splits, (unsigned)ny, (unsigned)nz);
-    if (p.c.fp8) k_attend<DP, NT, SPLIT, true><<<grid, kThreads, 0, s>>>(p, plan);
-    else k_attend<DP, NT, SPLIT, false><<<grid, kThreads, 0, s>>>(p, plan);
+cudaError_t launch2(const AttendParams &p, int sms, cudaStream_t s) {
+    constexpr int kBytes = Layout<DP, NT, SPLIT>::kBytes;
+    CUtensorMap k_map, v_map;
+    if (!codes_map(&k_map, p.c, p.c.k, DP, kBlk) || !codes_map(&v_map, p.c, p.c.v, DP, kBlk)) return cudaErrorInvalidValue;
+    auto kernel = p.c.fp8 ? k_attend<DP, NT, SPLIT, true> : k_attend<DP, NT, SPLIT, false>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess) return e;
+    // one wave; fewer CTAs when there are not four blocks (one per warp) for each
+    const long long rows = (long long)p.b.max_new * (p.q.heads / p.c.heads);
+    const long long items = (long long)p.b.n_seqs * p.c.heads * ((rows + 8 * NT - 1) / (8 * NT));
+    const long long blocks = p.b.max_len / kBlk + 2;
+    const long long most = std::min<long long>(items * ((blocks + kWarps - 1) / kWarps), kCounters);
+    const int grid = (int)std::min<long long>((long long)sms * ctas_per_sm<NT, SPLIT>(), most);
+    kernel<<<grid, kThreads, kBytes, s>>>(k_map, v_map, p);
     return cudaGetLastError();
 }
 
 template <int DP>
-cudaError_t launch1(const AttendParams &p, const Plan &plan, bool split_f32, cudaStream_t s) {
-    if (split_f32) return plan.nt == 1 ? launch2<DP, 1, true>(p, plan, s) : launch2<DP, 2, true>(p, plan, s);
-    return plan.nt == 1 ? launch2<DP, 1, false>(p, plan, s) : plan.nt == 2 ? launch2<DP, 2, false>(p, plan, s) : launch2<DP, 4, false>(p, plan, s);
-}
-
-size_t plan_bytes(const Cache &c, const Plan &p) {
-    if (p.splits <= 1) return 0;
-    const size_t dp = c.dim <= 64 ? 64 : 128;
-    return kCounters * sizeof(int) + (size_t)p.items * p.splits * (8 * p.nt) * (dp + 2) * sizeof(float);
+cudaError_t launch1(const AttendParams &p, int nt, bool split_f32, int sms, cudaStream_t s) {
+    if (split_f32) return nt == 1 ? launch2<DP, 1, true>(p, sms, s) : launch2<DP, 2, true>(p, sms, s);
+    return nt == 1 ? launch2<DP, 1, false>(p, sms, s) : nt == 2 ? launch2<DP, 2, false>(p, sms, s) : launch2<DP, 4, false>(p, sms, s);
 }
 
 }  // namespace
 
 size_t attend_workspace(const Cache &c, const Batch &b, int q_heads, int sms) {
-    return std::max(plan_bytes(c, plan_of(c, b, q_heads, sms, false, b.max_len)),
-                    plan_bytes(c, plan_of(c, b, q_heads, sms, true, b.max_len)));
+    size_t floats = 0;
+    for (bool split_f32 : {false, true}) {
+        const int nt = tiles_of(c, b.max_new, q_heads, split_f32);
+        const size_t ctas = std::min<size_t>((size_t)sms * (nt == 1 ? ctas_per_sm<1, false>() : ctas_per_sm<2, false>()), kCounters);
+        floats = std::max(floats, ctas * 2 * (8 * nt) * ((c.dim <= 64 ? 64 : 128) + 2));
+    }
+    return kCounters * sizeof(int) + floats * sizeof(float);
 }
 
 cudaError_t attend(const AttendParams &p, int sms, cudaStream_t s) {
     const bool split_f32 = p.out.dtype == kF32;
-    // keys that a row tile can see, at most; no more than the workspace was sized for
-    long long seen = p.b.max_len;
-    if (p.window) seen = std::min<long long>(seen, (long long)p.window + p.sinks + p.b.max_new);
-    const Plan plan = plan_of(p.c, p.b, p.q.heads, sms, split_f32, (int)seen);
-    return p.c.dim <= 64 ? launch1<64>(p, plan, split_f32, s) : launch1<128>(p, plan, split_f32, s);
+    const int nt = tiles_of(p.c, p.b.max_new, p.q.heads, split_f32);
+    return p.c.dim <= 64 ? launch1<64>(p, nt, split_f32, sms, s) : launch1<128>(p, nt, split_f32, sms, s);
 }
 
 }  // namespace kv

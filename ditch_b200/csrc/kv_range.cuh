@@ -26,25 +26,32 @@ __device__ __forceinline__ Range range_of(int lo, int hi, int window, int sinks,
     return r;
 }
 
-// Codes to f16, exactly. int8: the code + 128 goes into the mantissa of 1024
-// and 1152 is taken off again. E4M3: sign, exponent and mantissa move to
-// f16's places, which gives the value / 256 (f16's subnormals hold E4M3's);
-// the two NaN codes, which append never stores, count as +-480.
-__device__ __forceinline__ uint32_t int8_pair(uint32_t biased, uint32_t select) {
-    const uint32_t u = __byte_perm(biased, 0x64646464u, select);
+// Codes to f16, exactly. int8: the code + 128 goes into the mantissa of 1024,
+// and 1152 is taken off again, here or (where the products' sum can bear it)
+// from the sum. E4M3 by cvt, a pair at a time.
+constexpr float kInt8Bias = 1152.0f;
+
+__device__ __forceinline__ uint32_t int8_biased(uint32_t plus128, uint32_t select) {
+    return __byte_perm(plus128, 0x64646464u, select);
+}
+
+__device__ __forceinline__ uint32_t int8_pair(uint32_t plus128, uint32_t select) {
+    const uint32_t u = int8_biased(plus128, select);
     const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Codes in the upper bytes of the two halves (the lower bytes are ignored).
-__device__ __forceinline__ uint32_t e4m3_pair_f16(uint32_t u) { return ((u >> 1) & 0x3f803f80u) | (u & 0x80008000u); }
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t &a, uint32_t &b) {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(w));
+}
 
-// Four codes of one key: int8 as (0, 1) and (2, 3), E4M3 as (0, 2) and (1, 3).
+// Four codes as the pairs (0, 1) and (2, 3).
 template <bool FP8>
-__device__ __forceinline__ void key_pairs(uint32_t w, uint32_t &a, uint32_t &b) {
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t &a, uint32_t &b) {
     if (FP8) {
-        a = e4m3_pair_f16(w << 8);
-        b = e4m3_pair_f16(w);
+        e4m3_pairs(w, a, b);
     } else {
         w ^= 0x80808080u;
         a = int8_pair(w, 0x4140);
@@ -52,16 +59,17 @@ __device__ __forceinline__ void key_pairs(uint32_t w, uint32_t &a, uint32_t &b) 
     }
 }
 
-// Codes 2 half and 2 half + 1 of two tokens' four, each as a pair over the tokens.
-template <bool FP8>
+// Codes 2 half and 2 half + 1 of two tokens' four, each as a pair over the
+// tokens; int8 still biased by kInt8Bias when BIASED.
+template <bool FP8, bool BIASED>
 __device__ __forceinline__ void value_pairs(uint32_t w0, uint32_t w1, int half, uint32_t &a, uint32_t &b) {
-    const uint32_t u = __byte_perm(w0, w1, half ? 0x7362 : 0x5140);  // 0 of both, 1 of both
+    uint32_t u = __byte_perm(w0, w1, half ? 0x7362 : 0x5140);  // 0 of both, 1 of both
     if (FP8) {
-        a = e4m3_pair_f16(__byte_perm(u, 0, 0x1404));
-        b = e4m3_pair_f16(__byte_perm(u, 0, 0x3424));
+        e4m3_pairs(u, a, b);
     } else {
-        a = int8_pair(u ^ 0x80808080u, 0x4140);
-        b = int8_pair(u ^ 0x80808080u, 0x4342);
+        u ^= 0x80808080u;
+        a = BIASED ? int8_biased(u, 0x4140) : int8_pair(u, 0x4140);
+        b = BIASED ? int8_biased(u, 0x4342) : int8_pair(u, 0x4342);
     }
 }
 

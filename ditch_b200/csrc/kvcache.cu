@@ -1,6 +1,7 @@
 // Appending keys and values to the paged 8-bit cache, with the rotation of
 // queries and keys on the way, and reading tokens back as rows.
-#include "kv_range.cuh"
+#include "gemm.cuh"
+#include "kvcache.cuh"
 
 namespace ditch {
 namespace kv {
@@ -131,9 +132,8 @@ __device__ __forceinline__ uint2 encode8(bool fp8, const float (&x)[8], float f)
 
 __device__ __forceinline__ void decode4(bool fp8, uint32_t u, float *x) {
     if (fp8) {
-        uint32_t even = e4m3_pair_f16(u << 8), odd = e4m3_pair_f16(u);
-        const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&even)), b = __half22float2(*reinterpret_cast<__half2 *>(&odd));
-        x[0] = a.x * 256.0f, x[1] = b.x * 256.0f, x[2] = a.y * 256.0f, x[3] = b.y * 256.0f;
+        const float2 a = e4m3x2_f32(u & 0xffff), b = e4m3x2_f32(u >> 16);
+        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] = static_cast<float>(static_cast<int8_t>(u >> (8 * i)));
@@ -339,6 +339,15 @@ __global__ void __launch_bounds__(256) k_kv_read(ReadParams p) {
 }
 
 }  // namespace
+
+bool codes_map(CUtensorMap *map, const Cache &c, const void *codes, int row_bytes, int tokens) {
+    const cuuint64_t page = (cuuint64_t)c.heads << c.page_shift;
+    const cuuint64_t dims[3] = {(cuuint64_t)c.dim, page, (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.dim, page * c.dim};
+    const cuuint32_t box[3] = {(cuuint32_t)row_bytes, (cuuint32_t)tokens, 1};
+    return tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, codes, dims, strides, box,
+                      row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
 
 cudaError_t append(const AppendParams &p, cudaStream_t s) {
     const int lpt = p.c.dim <= 32 ? 2 : p.c.dim <= 64 ? 4 : 8;

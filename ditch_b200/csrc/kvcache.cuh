@@ -74,6 +74,11 @@ struct WindowParams {
     int *status;
 };
 
+// The tensor map of a pool's K or V codes for boxes of `tokens` tokens of one
+// page and head: rows of row_bytes (64 or 128) with as wide a swizzle, zeros
+// past the head's dimensions. Coordinates (0, head * page_tokens + t, page).
+bool codes_map(CUtensorMap *map, const Cache &c, const void *codes, int row_bytes, int tokens);
+
 cudaError_t append(const AppendParams &p, cudaStream_t s);
 cudaError_t read_back(const ReadParams &p, cudaStream_t s);
 size_t attend_workspace(const Cache &c, const Batch &b, int q_heads, int sms);
@@ -137,6 +142,19 @@ __device__ __forceinline__ void store1(const Rows &r, long long at, float v) {
     if (r.dtype == kF32) static_cast<float *>(r.p)[at] = v;
     else if (r.dtype == kBf16) static_cast<uint16_t *>(r.p)[at] = f32_to_bf16_bits(v);
     else static_cast<__half *>(r.p)[at] = __float2half_rn(v);
+}
+
+// Four values to a 16-byte aligned row, at a multiple of four.
+__device__ __forceinline__ void store4(const Rows &r, long long at, float4 v) {
+    if (r.dtype == kF32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(r.p) + at) = v;
+    } else if (r.dtype == kBf16) {
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(r.p) + at) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    } else {
+        const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(r.p) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
 }
 
 }  // namespace kv

@@ -397,7 +397,7 @@ int ditch_cuda_edit_weight_bf16_noalloc(void *w, size_t rows, size_t cols, const
  * or a page outside its bounds) is left out and sets the device's status
  * word: the next ditch_cuda_synchronize returns DITCH_CUDA_INVALID. */
 #define DITCH_KV_INT8 0 /* codes -127..127 */
-#define DITCH_KV_FP8 1  /* codes E4M3 (largest 448; the NaN codes are never stored and read as +-480) */
+#define DITCH_KV_FP8 1  /* codes E4M3 (largest 448; its NaN codes are never stored) */
 
 /* A pool of pages for one layer. A page holds page_tokens consecutive tokens
  * of one sequence; every block_tokens of them share one scale per kv head:
@@ -468,14 +468,14 @@ int ditch_cuda_kv_read(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache,
  * j <= p and (window is 0, or j > p - window, or j < sinks):
  * out = sum softmax(scale * q . k) v, zero for a row that sees nothing. Query
  * head h reads kv head h / (heads / kv_heads). What a row does not see does
- * not change it, whatever its codes; a scale that is not finite makes
- * the rows that see its block not finite. f32 out is computed to f32
+ * not change it (E4M3's NaN codes within its sequence excepted); a scale that
+ * is not finite makes the rows that see its block not finite. f32 out is computed to f32
  * rounding, f16 and bf16 out with the softmax weights rounded to f16. The
  * workspace holds the partial sums of sequences split over the GPU: at least
  * ditch_cuda_kv_attention_workspace bytes for the same cache, batch sizes and
- * query heads (0: none is needed), 16-byte aligned, zero-filled before its
- * first use and then left to these calls, one at a time; it may serve batches
- * of other sizes that fit. */
+ * query heads (0: none is needed, or an argument is wrong), 16-byte aligned,
+ * zero-filled before its first use and then left to these calls, one at a
+ * time (of any batch that it is large enough for). */
 size_t ditch_cuda_kv_attention_workspace(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache,
                                          const ditch_cuda_kv_batch *batch, size_t q_heads);
 int ditch_cuda_kv_attention(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache, const ditch_cuda_kv_batch *batch,
