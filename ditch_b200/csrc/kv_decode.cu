@@ -12,17 +12,22 @@
 // with the block's scales applied to the f32 products: s = sk c_r S^T where
 // c_r holds the softmax scale and the power of two by which row r of Q was
 // brought into f16's range, and sv as the block's P . V is added to the f32
-// sums. Each warp keeps a ring of blocks of its own in shared memory, filled
-// by TMA three blocks ahead (a box of 16 tokens, rows padded with zeros to 64
-// or 128 bytes, swizzled so that the reads below meet no bank twice), and
-// waits for nobody else. The order of the reduction is free, so a lane's 32
+// sums. int8 keys are not converted at all: Q is taken as a 23-bit fixed-point
+// number of three signed 8-bit digits and multiplied with m16n8k32 integer
+// MMAs, exactly (three MMAs for what would be two in f16, but no work per
+// code). Each warp keeps a ring of pairs of blocks of its own in shared
+// memory, filled by TMA one pair ahead (a box of 16 tokens, rows padded with
+// zeros to 64 or 128 bytes, swizzled so that the reads below meet no bank
+// twice), and waits for nobody else. Two blocks at a time give the chains of
+// dependent MMAs company. The order of the reduction is free, so a lane's 32
 // (of K) or 16 (of V) contiguous dimensions are the ones its fragments name.
 //
 // Online softmax per warp in base 2. The reference maximum moves only when a
 // score passes it by kLazy: weights stay below 2^kLazy, well inside f16, and
 // most blocks skip the reduction over the lanes and the rescale.
 //
-// f32 rows: Q and P are each split into two f16 (22 bits), two MMAs for one.
+// f32 rows: P (and Q over an E4M3 cache) is split into two f16 (22 bits), two
+// MMAs for one.
 //
 // The blocks of all work items (sequence, key / value head, row tile), one
 // item after another, are divided evenly over as many CTAs as the GPU holds,
@@ -41,7 +46,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kBlk = 16;         // tokens of one step of a warp
+constexpr int kBlk = 16;         // tokens of a block: what one MMA takes
+constexpr int kMinBlocks = 4;    // of a CTA's share
 constexpr float kLazy = 8.0f;
 constexpr int kCounters = 4096;  // arrival counters (one per CTA), first in the workspace
 constexpr float kLog2e = 1.4426950408889634f;
@@ -49,6 +55,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
@@ -71,10 +83,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// A warp's ring: kDepth blocks of K and V codes, rows of DP bytes swizzled by
+// A warp's ring: kDepth pairs of blocks of K and V codes, rows of DP bytes swizzled by
 // TMA (16-byte chunk c of row r lies at c ^ (r & 7) for 128-byte rows, at
 // c ^ (r / 2 & 3) for 64-byte rows).
-constexpr int kDepth = 3;
+constexpr int kDepth = 2;
 
 template <int DP>
 __device__ __forceinline__ const uint8_t *chunk_of(const uint8_t *tile, int r, int c) {
@@ -109,7 +121,7 @@ struct Smem {
 // CTAs of four warps to an SM, by their registers.
 template <int NT, bool SPLIT>
 constexpr int ctas_per_sm() {
-    return NT == 1 ? (SPLIT ? 3 : 4) : 2;
+    return NT == 1 ? 3 : 2;
 }
 
 // Shared memory from a 1024-byte aligned base: the rings, over which the
@@ -117,9 +129,11 @@ constexpr int ctas_per_sm() {
 template <int DP, int NT, bool SPLIT>
 struct Layout {
     static constexpr int kTile = kBlk * DP;  // bytes of a block's K or V
-    static constexpr int kRing = kWarps * kDepth * 2 * kTile;
+    static constexpr int kStage = 4 * kTile;  // K, V of the first block, K, V of the second
+    static constexpr int kRing = kWarps * kDepth * kStage;
     static constexpr int kO = kWarps * 8 * NT * DP * 4;
-    static constexpr int kQ = (SPLIT ? 2 : 1) * 8 * NT * (DP + 8) * 2;
+    static constexpr int kQf16 = (SPLIT ? 2 : 1) * 8 * NT * (DP + 8) * 2, kQdigits = 3 * 8 * NT * (DP + 16);
+    static constexpr int kQ = kQf16 > kQdigits ? kQf16 : kQdigits;
     static constexpr int kQAt = kRing > kO ? kRing : kO;
     static constexpr int kBytes = 1024 + kQAt + kQ;
 };
@@ -153,7 +167,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     using L = Layout<DP, NT, SPLIT>;
     constexpr int kRows = 8 * NT;
     constexpr int kQs = DP + 8;        // row stride of Q in shared memory (f16)
-    constexpr int kSteps = DP / 16;    // MMA steps over the dimensions
+    constexpr int kQd = DP + 16;       // row stride of Q's digits (bytes)
+    constexpr int kSteps = FP8 ? DP / 16 : DP / 32;  // MMA steps over the dimensions
+    constexpr bool kQRegs = NT == 1 && (!SPLIT || !FP8);  // Q's fragments stay in registers
+    constexpr int kDigits = FP8 ? 1 : 3;
     constexpr int kMt = DP / 16;       // tiles of 16 dimensions of O^T
     constexpr bool kBiased = !FP8 && !SPLIT;  // V codes + 1152: see below
     constexpr int kPart = kRows * (DP + 2);   // floats of a part: sums, maxima, sums of weights
@@ -164,7 +181,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     __half *s_q = reinterpret_cast<__half *>(base + L::kQAt);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int group = p.q.heads / p.c.heads;
-    uint8_t *ring = base + warp * (kDepth * 2 * L::kTile);
+    int8_t *s_d = reinterpret_cast<int8_t *>(s_q);
+    uint8_t *ring = base + warp * (kDepth * L::kStage);
     uint64_t *full = sm.full[warp];
     if (lane == 0) {
         for (int i = 0; i < kDepth; i++) mbar_init(&full[i], 1);
@@ -194,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         if (w < warp) upto += sm.sums[w];
         total += sm.sums[w];
     }
-    const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kWarps));
+    const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinBlocks));
     long long pos = per * blockIdx.x;
     const long long end = min(total, pos + per);
     if (pos >= end) return;
@@ -230,42 +248,63 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         const Range range = range_of(p_lo, p_hi, p.window, p.sinks, kBlk);
         const int b_lo = off, b_hi = min(range.n, off + n_slots);
 
-        // ---- this warp's blocks: b_lo + warp, + kWarps, ...; lane i looks up the page of the i-th ----
-        int ahead = 0, pages = -1;
-        auto look_up = [&]() {
-            const int x = b_lo + warp + kWarps * (ahead + lane);
-            pages = x < b_hi ? page_of(p.c, p.b, seq, range.token(x, kBlk), p.status) : -1;
-        };
-        look_up();
-        // a block under way: its first token (-1: nothing to see) and scales
-        struct Under {
-            int tok;
+        // ---- this warp's pairs of blocks: b_lo + 2 (warp + 4 i), + 1; lane 2 j + u looks up the
+        // page and scales of block u of the (ahead + j)-th pair, half a window before they are used ----
+        struct Look {
+            int page;
             float sk, sv;
         };
+        auto look_up = [&](int from) {
+            Look k;
+            const int x = b_lo + 2 * (warp + kWarps * (from + (lane >> 1))) + (lane & 1);
+            const int tok = range.token(x, kBlk);
+            k.page = x < b_hi ? page_of(p.c, p.b, seq, tok, p.status) : -1;
+            k.sk = k.sv = 0.0f;
+            if (k.page >= 0) {
+                const long long sa = scale_at(p.c, k.page, head, tok);
+                k.sk = __ldg(p.c.ks + sa);
+                k.sv = __ldg(p.c.vs + sa);
+            }
+            return k;
+        };
+        int ahead = 0;
+        Look look = look_up(0), later;
+        later.page = -1;
+        // a pair under way: first tokens (-1: nothing to see) and scales
+        struct Under {
+            int tok[2];
+            float sk[2], sv[2];
+        };
         auto fetch = [&](int stage, int i) {
+            if (i - ahead == 8) later = look_up(ahead + 16);
+            if (i - ahead == 16) {
+                ahead += 16;
+                look = later;
+            }
             Under u;
-            u.tok = -1;
-            u.sk = u.sv = 0.0f;
-            if (i - ahead >= 32) {
-                ahead += 32;
-                look_up();
+            int page[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int from = 2 * (i - ahead) + h;
+                page[h] = __shfl_sync(0xffffffffu, look.page, from);
+                u.sk[h] = __shfl_sync(0xffffffffu, look.sk, from);
+                u.sv[h] = __shfl_sync(0xffffffffu, look.sv, from);
+                u.tok[h] = page[h] < 0 ? -1 : range.token(b_lo + 2 * (warp + kWarps * i) + h, kBlk);
             }
-            const int page = __shfl_sync(0xffffffffu, pages, i - ahead);
-            if (page < 0) return u;
-            u.tok = range.token(b_lo + warp + kWarps * i, kBlk);
-            if (lane == 0) {
-                uint8_t *tile_at = ring + stage * 2 * L::kTile;
-                const int y = (head << p.c.page_shift) + (u.tok & page_mask);
-                mbar_arrive_expect_tx(&full[stage], 2 * L::kTile);
-                tma_load_3d(&k_map, &full[stage], tile_at, y, page);
-                tma_load_3d(&v_map, &full[stage], tile_at + L::kTile, y, page);
+            const int n = (page[0] >= 0) + (page[1] >= 0);
+            if (n && lane == 0) {
+                uint8_t *at = ring + stage * L::kStage;
+                mbar_arrive_expect_tx(&full[stage], n * 2 * L::kTile);
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (page[h] >= 0) {
+                        const int y = (head << p.c.page_shift) + (u.tok[h] & page_mask);
+                        tma_load_3d(&k_map, &full[stage], at + 2 * h * L::kTile, y, page[h]);
+                        tma_load_3d(&v_map, &full[stage], at + (2 * h + 1) * L::kTile, y, page[h]);
+                    }
             }
-            const long long sa = scale_at(p.c, page, head, u.tok);
-            u.sk = __ldg(p.c.ks + sa);
-            u.sv = __ldg(p.c.vs + sa);
             return u;
         };
-        auto next = [](int s) { return s + 1 == kDepth ? 0 : s + 1; };
 
         // ---- Q rows into registers, the first blocks under way, Q to f16 ----
         float qx[kRows / kWarps][DP / 32];
@@ -279,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                 qx[i][e] = r < n_rows && d < p.c.dim ? load1(p.q, at + d) : 0.0f;
             }
         }
-        Under u0 = fetch(st, 0), u1 = fetch(next(st), 1), u2 = fetch(next(next(st)), 2);
+        Under u0 = fetch(st, 0), u1 = fetch(st ^ 1, 1);
 #pragma unroll
         for (int i = 0; i < kRows / kWarps; i++) {  // each row by a power of two to below 2
             const int r = warp + kWarps * i;
@@ -290,14 +329,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             int e2 = static_cast<int>(top >> 23) - 127;
             e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
             const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
-            if (lane == 0) s_c[r] = p.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+            if (lane == 0) {
+                float c = p.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+                if (!FP8) c = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : c * 0x1p-21f;
+                s_c[r] = c;
+            }
 #pragma unroll
             for (int e = 0; e < DP / 32; e++) {
                 const int d = lane + 32 * e;
                 const float y = qx[i][e] * down;
-                const __half h = __float2half_rn(y);
-                s_q[r * kQs + d] = h;
-                if (SPLIT) s_q[(kRows + r) * kQs + d] = __float2half_rn(y - __half2float(h));
+                if (FP8) {
+                    const __half h = __float2half_rn(y);
+                    s_q[r * kQs + d] = h;
+                    if (SPLIT) s_q[(kRows + r) * kQs + d] = __float2half_rn(y - __half2float(h));
+                } else {  // |y| < 2: 23 bits, digits of the sum 65536 d2 + 256 d1 + d0
+                    const int v = __float2int_rn(y * 0x1p21f);
+                    const int d0 = static_cast<int8_t>(v), v1 = (v - d0) >> 8, d1 = static_cast<int8_t>(v1);
+                    s_d[r * kQd + d] = static_cast<int8_t>(d0);
+                    s_d[(kRows + r) * kQd + d] = static_cast<int8_t>(d1);
+                    s_d[(2 * kRows + r) * kQd + d] = static_cast<int8_t>((v1 - d1) >> 8);
+                }
             }
         }
         __syncthreads();
@@ -313,14 +364,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                 top_key[n][e] = r < n_rows ? first + (r0 + r) / group : -1;
                 low_key[n][e] = p.window ? top_key[n][e] - p.window + 1 : 0;
             }
-        uint32_t qf[NT == 1 && !SPLIT ? kSteps : 1][2];
-        if (NT == 1 && !SPLIT) {
+        auto q_frag = [&](int n, int step, int part) {  // part: low half of SPLIT's f16, or the digit
+            return FP8 ? *reinterpret_cast<const uint2 *>(s_q + (part * kRows + 8 * n + g) * kQs + t * (DP / 4) + 4 * step)
+                       : *reinterpret_cast<const uint2 *>(s_d + (part * kRows + 8 * n + g) * kQd + t * (DP / 4) + 8 * step);
+        };
+        uint2 qf[kQRegs ? kSteps : 1][kDigits];
+        if (kQRegs) {
 #pragma unroll
-            for (int s = 0; s < kSteps; s++) {
-                const uint2 u = *reinterpret_cast<const uint2 *>(s_q + g * kQs + t * (DP / 4) + 4 * s);
-                qf[NT == 1 && !SPLIT ? s : 0][0] = u.x;
-                qf[NT == 1 && !SPLIT ? s : 0][1] = u.y;
-            }
+            for (int s = 0; s < kSteps; s++)
+#pragma unroll
+                for (int d = 0; d < kDigits; d++) qf[kQRegs ? s : 0][d] = q_frag(0, s, d);
         }
 
         float o[NT][kMt][4], m[NT][2], l[NT][2];
@@ -335,77 +388,116 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         }
 
         auto use = [&](int stage, const Under &s) {
-            if (s.tok < 0 || dead) return;
+            if ((s.tok[0] < 0 && s.tok[1] < 0) || dead) return;
             if (!mbar_wait(&full[stage], (phase >> stage) & 1, &sm.abort, p.status)) {
                 dead = true;
                 return;
             }
             phase ^= 1u << stage;
-            const uint8_t *kt = ring + stage * 2 * L::kTile, *vt = kt + L::kTile;
+            const uint8_t *tiles = ring + stage * L::kStage;
             // ---- S^T = K . Q^T ----
-            // (even and odd steps apart: two chains of dependent MMAs)
-            float sc[NT][4], odd[NT][4];
+            float sc[2][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int u = 0; u < 2; u++) {
+                const uint8_t *kt = tiles + 2 * u * L::kTile;
+                uint32_t w0[DP / 16], w1[DP / 16];  // tokens g and g + 8, dimensions (DP / 4) t ...
 #pragma unroll
-                for (int e = 0; e < 4; e++) sc[n][e] = odd[n][e] = 0.0f;
+                for (int i = 0; i < DP / 64; i++) {
+                    const uint4 k0 = *reinterpret_cast<const uint4 *>(chunk_of<DP>(kt, g, t * (DP / 64) + i));
+                    const uint4 k1 = *reinterpret_cast<const uint4 *>(chunk_of<DP>(kt, g + 8, t * (DP / 64) + i));
+                    w0[4 * i] = k0.x, w0[4 * i + 1] = k0.y, w0[4 * i + 2] = k0.z, w0[4 * i + 3] = k0.w;
+                    w1[4 * i] = k1.x, w1[4 * i + 1] = k1.y, w1[4 * i + 2] = k1.z, w1[4 * i + 3] = k1.w;
+                }
+                if constexpr (FP8) {
+                    // (even and odd steps apart: two chains of dependent MMAs)
+                    float odd[NT][4];
 #pragma unroll
-            for (int i = 0; i < DP / 64; i++) {
-                const uint4 k0 = *reinterpret_cast<const uint4 *>(chunk_of<DP>(kt, g, t * (DP / 64) + i));
-                const uint4 k1 = *reinterpret_cast<const uint4 *>(chunk_of<DP>(kt, g + 8, t * (DP / 64) + i));
-                const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+                    for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t f[4];
-                    code_pairs<FP8>(w0[j], f[0], f[2]);
-                    code_pairs<FP8>(w1[j], f[1], f[3]);
-                    const int step = 4 * i + j;
+                        for (int e = 0; e < 4; e++) sc[u][n][e] = odd[n][e] = 0.0f;
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        float(&acc)[4] = step & 1 ? odd[n] : sc[n];
-                        if (NT == 1 && !SPLIT) {
-                            mma_f16(acc, f, qf[NT == 1 && !SPLIT ? step : 0][0], qf[NT == 1 && !SPLIT ? step : 0][1]);
-                        } else {
-                            const __half *at = s_q + (8 * n + g) * kQs + t * (DP / 4) + 4 * step;
-                            const uint2 u = *reinterpret_cast<const uint2 *>(at);
-                            mma_f16(acc, f, u.x, u.y);
+                    for (int i = 0; i < kSteps; i++) {
+                        uint32_t f[4];
+                        e4m3_pairs(w0[i], f[0], f[2]);
+                        e4m3_pairs(w1[i], f[1], f[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            float(&acc)[4] = i & 1 ? odd[n] : sc[u][n];
+                            const uint2 b = kQRegs ? qf[kQRegs ? i : 0][0] : q_frag(n, i, 0);
+                            mma_f16(acc, f, b.x, b.y);
                             if (SPLIT) {
-                                const uint2 w = *reinterpret_cast<const uint2 *>(at + kRows * kQs);
-                                mma_f16(acc, f, w.x, w.y);
+                                const uint2 low = q_frag(n, i, 1);
+                                mma_f16(acc, f, low.x, low.y);
                             }
                         }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sc[u][n][e] += odd[n][e];
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        int acc[3][4];
+#pragma unroll
+                        for (int d = 0; d < 3; d++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[d][e] = 0;
+#pragma unroll
+                        for (int i = 0; i < kSteps; i++) {
+                            const uint32_t f[4] = {w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1]};
+#pragma unroll
+                            for (int d = 0; d < 3; d++) {
+                                const uint2 b = kQRegs ? qf[kQRegs ? i : 0][FP8 ? 0 : d] : q_frag(n, i, d);
+                                mma_s8(acc[d], f, b.x, b.y);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            sc[u][n][e] = fmaf(static_cast<float>(acc[2][e] * 256 + acc[1][e]), 256.0f, static_cast<float>(acc[0][e]));
                     }
                 }
             }
             // ---- softmax ----
-            const bool whole = s.tok + kBlk - 1 <= p_lo && (!p.window || s.tok > p_hi - p.window);
-            bool sees[NT][2];
+            bool whole[2], sees[2][NT][2];
             bool over = false;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int u = 0; u < 2; u++) {
+                whole[u] = s.tok[u] >= 0 && s.tok[u] + kBlk - 1 <= p_lo && (!p.window || s.tok[u] > p_hi - p.window);
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float f = s.sk * c_row[n][e];
-                    sc[n][e] = (sc[n][e] + odd[n][e]) * f;
-                    sc[n][e + 2] = (sc[n][e + 2] + odd[n][e + 2]) * f;
-                    sees[n][e] = true;
-                    if (!whole) {
-                        const int hi = top_key[n][e], lo = low_key[n][e];
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int key = s.tok + g + 8 * h;
-                            if (key > hi || (key < lo && key >= p.sinks)) sc[n][e + 2 * h] = -INFINITY;
-                        }
-                        sees[n][e] = s.tok <= hi && (s.tok + kBlk > lo || s.tok < p.sinks);
+                    for (int e = 0; e < 2; e++) {
+                        const float f = s.sk[u] * c_row[n][e];
+                        sc[u][n][e] *= f;
+                        sc[u][n][e + 2] *= f;
+                        sees[u][n][e] = true;
                     }
-                    over |= fmaxf(sc[n][e], sc[n][e + 2]) > m[n][e] + kLazy;
+                if (!whole[u]) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int hi = s.tok[u] < 0 ? -2 : top_key[n][e], lo = low_key[n][e];
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const int key = s.tok[u] + g + 8 * h;
+                                if (key > hi || (key < lo && key >= p.sinks)) sc[u][n][e + 2 * h] = -INFINITY;
+                            }
+                            sees[u][n][e] = s.tok[u] <= hi && (s.tok[u] + kBlk > lo || s.tok[u] < p.sinks);
+                        }
                 }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) over |= fmaxf(sc[u][n][e], sc[u][n][e + 2]) > m[n][e] + kLazy;
+            }
             if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float x = fmaxf(sc[n][e], sc[n][e + 2]);
+                        float x = fmaxf(fmaxf(sc[0][n][e], sc[0][n][e + 2]), fmaxf(sc[1][n][e], sc[1][n][e + 2]));
 #pragma unroll
                         for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
                         x = fmaxf(x, m[n][e]);
@@ -419,90 +511,92 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                         }
                     }
             }
-            uint32_t pb[NT][2], pl[SPLIT ? NT : 1][2];
+            uint32_t pb[2][NT][2], pl[2][SPLIT ? NT : 1][2];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float ref = m[n][e] == -INFINITY ? 0.0f : m[n][e];
-                    sc[n][e] = exp2_fast(sc[n][e] - ref);
-                    sc[n][e + 2] = exp2_fast(sc[n][e + 2] - ref);
-                    l[n][e] += sc[n][e] + sc[n][e + 2];
-                }
+                for (int n = 0; n < NT; n++) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t u = half2_bits(sc[n][2 * h], sc[n][2 * h + 1]);
-                    pb[n][h] = transpose8x8(u);
-                    if (SPLIT) {
-                        const float2 f = half2_floats(u);
-                        pl[SPLIT ? n : 0][h] = transpose8x8(half2_bits(sc[n][2 * h] - f.x, sc[n][2 * h + 1] - f.y));
+                    for (int e = 0; e < 2; e++) {
+                        const float ref = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+                        sc[u][n][e] = exp2_fast(sc[u][n][e] - ref);
+                        sc[u][n][e + 2] = exp2_fast(sc[u][n][e + 2] - ref);
+                        l[n][e] += sc[u][n][e] + sc[u][n][e + 2];
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t b = half2_bits(sc[u][n][2 * h], sc[u][n][2 * h + 1]);
+                        pb[u][n][h] = transpose8x8(b);
+                        if (SPLIT) {
+                            const float2 f = half2_floats(b);
+                            pl[u][SPLIT ? n : 0][h] = transpose8x8(half2_bits(sc[u][n][2 * h] - f.x, sc[u][n][2 * h + 1] - f.y));
+                        }
                     }
                 }
-            }
             // ---- O^T += sv V^T . P^T ----
             // Biased codes: the sums start at -1152 sum(P), from an MMA with the
             // same rounded P, so the bias cancels within the block's f32 sum (an
             // error of 2^-23 of 1152 sum(P), about 1e-5 of a typical block's).
-            float zero[NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+            for (int u = 0; u < 2; u++) {
+                const uint8_t *vt = tiles + (2 * u + 1) * L::kTile;
+                float zero[NT][4], w[NT][2];
 #pragma unroll
-                for (int e = 0; e < 4; e++) zero[n][e] = 0.0f;
-                const uint32_t minus[4] = {0xe480e480u, 0xe480e480u, 0xe480e480u, 0xe480e480u};
-                if (kBiased) mma_f16(zero[n], minus, pb[n][0], pb[n][1]);
-            }
-            float w[NT][2];
+                for (int n = 0; n < NT; n++) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+                    for (int e = 0; e < 4; e++) zero[n][e] = 0.0f;
+                    const uint32_t minus[4] = {0xe480e480u, 0xe480e480u, 0xe480e480u, 0xe480e480u};
+                    if (kBiased) mma_f16(zero[n], minus, pb[u][n][0], pb[u][n][1]);
 #pragma unroll
-                for (int e = 0; e < 2; e++) w[n][e] = sees[n][e] ? s.sv : 0.0f;
-            // (an E4M3 NaN in memory past the sequence must not meet a weight of 0)
-            const int seen = whole || !FP8 ? kBlk : p_hi + 1 - s.tok;
-            uint32_t v[4][DP / 32];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9, dimensions (DP / 8) g ...
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int tok = 2 * t + (r & 1) + 8 * (r >> 1);
-                if (DP == 128) {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(chunk_of<DP>(vt, tok, g));
-                    v[r][0] = u.x, v[r][1] = u.y, v[r][DP / 32 - 2] = u.z, v[r][DP / 32 - 1] = u.w;
-                } else {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(chunk_of<DP>(vt, tok, g >> 1) + 8 * (g & 1));
-                    v[r][0] = u.x, v[r][1] = u.y;
+                    for (int e = 0; e < 2; e++) w[n][e] = sees[u][n][e] ? s.sv[u] : 0.0f;
                 }
-                if (FP8 && tok >= seen) {
+                // (an E4M3 NaN in memory past the sequence must not meet a weight of 0)
+                const int seen = whole[u] || !FP8 ? kBlk : s.tok[u] < 0 ? 0 : p_hi + 1 - s.tok[u];
+                uint32_t v[4][DP / 32];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9, dimensions (DP / 8) g ...
 #pragma unroll
-                    for (int i = 0; i < DP / 32; i++) v[r][i] = 0;
+                for (int r = 0; r < 4; r++) {
+                    const int tok = 2 * t + (r & 1) + 8 * (r >> 1);
+                    if (DP == 128) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(chunk_of<DP>(vt, tok, g));
+                        v[r][0] = x.x, v[r][1] = x.y, v[r][DP / 32 - 2] = x.z, v[r][DP / 32 - 1] = x.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(chunk_of<DP>(vt, tok, g >> 1) + 8 * (g & 1));
+                        v[r][0] = x.x, v[r][1] = x.y;
+                    }
+                    if (FP8 && tok >= seen) {
+#pragma unroll
+                        for (int i = 0; i < DP / 32; i++) v[r][i] = 0;
+                    }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < DP / 32; i++) {
+                for (int i = 0; i < DP / 32; i++) {
 #pragma unroll
-                for (int half = 0; half < 2; half++) {  // dimensions (DP / 8) g + 4 i + 2 half, + 1
-                    uint32_t f[4];
-                    value_pairs<FP8, kBiased>(v[0][i], v[1][i], half, f[0], f[1]);
-                    value_pairs<FP8, kBiased>(v[2][i], v[3][i], half, f[2], f[3]);
-                    const int j = 2 * i + half;
+                    for (int half = 0; half < 2; half++) {  // dimensions (DP / 8) g + 4 i + 2 half, + 1
+                        uint32_t f[4];
+                        value_pairs<FP8, kBiased>(v[0][i], v[1][i], half, f[0], f[1]);
+                        value_pairs<FP8, kBiased>(v[2][i], v[3][i], half, f[2], f[3]);
+                        const int j = 2 * i + half;
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        float x[4] = {zero[n][0], zero[n][1], zero[n][2], zero[n][3]};
-                        mma_f16(x, f, pb[n][0], pb[n][1]);
-                        if (SPLIT) mma_f16(x, f, pl[SPLIT ? n : 0][0], pl[SPLIT ? n : 0][1]);
-                        fma2(o[n][j][0], o[n][j][1], x[0], x[1], w[n][0], w[n][1]);
-                        fma2(o[n][j][2], o[n][j][3], x[2], x[3], w[n][0], w[n][1]);
+                        for (int n = 0; n < NT; n++) {
+                            float x[4] = {zero[n][0], zero[n][1], zero[n][2], zero[n][3]};
+                            mma_f16(x, f, pb[u][n][0], pb[u][n][1]);
+                            if (SPLIT) mma_f16(x, f, pl[u][SPLIT ? n : 0][0], pl[u][SPLIT ? n : 0][1]);
+                            fma2(o[n][j][0], o[n][j][1], x[0], x[1], w[n][0], w[n][1]);
+                            fma2(o[n][j][2], o[n][j][3], x[2], x[3], w[n][0], w[n][1]);
+                        }
                     }
                 }
             }
         };
 
-        const int n_steps = b_lo + warp < b_hi ? (b_hi - b_lo - warp + kWarps - 1) / kWarps : 0;
+        const int n_pairs = (b_hi - b_lo + 1) / 2, n_steps = warp < n_pairs ? (n_pairs - warp + kWarps - 1) / kWarps : 0;
 #pragma unroll 1
         for (int i = 0; i < n_steps; i++) {
             use(st, u0);
             __syncwarp();  // every lane has read the stage
             u0 = u1;
-            u1 = u2;
-            u2 = fetch(st, i + kDepth);
-            st = next(st);
+            u1 = fetch(st, i + kDepth);
+            st ^= 1;
         }
         if (dead) {  // give the loads in flight their time before the memory goes to others
             for (int x = 0; x < kDepth; x++) mbar_try_wait(&full[x], (phase >> x) & 1);
@@ -656,11 +750,11 @@ cudaError_t launch2(const AttendParams &p, int sms, cudaStream_t s) {
     auto kernel = p.c.fp8 ? k_attend<DP, NT, SPLIT, true> : k_attend<DP, NT, SPLIT, false>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (e != cudaSuccess) return e;
-    // one wave; fewer CTAs when there are not four blocks (one per warp) for each
+    // one wave; fewer CTAs when there are not kMinBlocks for each
     const long long rows = (long long)p.b.max_new * (p.q.heads / p.c.heads);
     const long long items = (long long)p.b.n_seqs * p.c.heads * ((rows + 8 * NT - 1) / (8 * NT));
     const long long blocks = p.b.max_len / kBlk + 2;
-    const long long most = std::min<long long>(items * ((blocks + kWarps - 1) / kWarps), kCounters);
+    const long long most = std::min<long long>(items * ((blocks + kMinBlocks - 1) / kMinBlocks), kCounters);
     const int grid = (int)std::min<long long>((long long)sms * ctas_per_sm<NT, SPLIT>(), most);
     kernel<<<grid, kThreads, kBytes, s>>>(k_map, v_map, p);
     return cudaGetLastError();

@@ -47,18 +47,6 @@ __device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t &a, uint32_t &b)
         : "r"(w));
 }
 
-// Four codes as the pairs (0, 1) and (2, 3).
-template <bool FP8>
-__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t &a, uint32_t &b) {
-    if (FP8) {
-        e4m3_pairs(w, a, b);
-    } else {
-        w ^= 0x80808080u;
-        a = int8_pair(w, 0x4140);
-        b = int8_pair(w, 0x4342);
-    }
-}
-
 // Codes 2 half and 2 half + 1 of two tokens' four, each as a pair over the
 // tokens; int8 still biased by kInt8Bias when BIASED.
 template <bool FP8, bool BIASED>
