@@ -34,7 +34,9 @@
 // whatever the sequences' lengths. A CTA's share may begin and end inside an
 // item: it leaves that item's sums (f32) in the workspace, and the CTA that
 // brings an item's last part adds the parts in order, so results do not
-// depend on timing.
+// depend on timing. Many short items (kernel parameter solo) are instead taken
+// whole, one by each warp, which needs neither: no sums to add, no waiting for
+// other warps.
 #include <algorithm>
 
 #include "gemm.cuh"
@@ -47,15 +49,16 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kBlk = 16;         // tokens of a block: what one MMA takes
-constexpr int kMinBlocks = 4;    // of a CTA's share
+constexpr int kMinBlocks = 8;    // of a CTA's share: a pair for each warp
 constexpr float kLazy = 8.0f;
 constexpr int kCounters = 4096;  // arrival counters (one per CTA), first in the workspace
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a b + c
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -89,8 +92,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 constexpr int kDepth = 2;
 
 template <int DP>
-__device__ __forceinline__ const uint8_t *chunk_of(const uint8_t *tile, int r, int c) {
-    return tile + r * DP + ((DP == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+    return r * DP + ((DP == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
 }
 
 __device__ __forceinline__ void tma_load_3d(const CUtensorMap *map, uint64_t *bar, void *dst, int y, int z) {
@@ -101,14 +104,39 @@ __device__ __forceinline__ void tma_load_3d(const CUtensorMap *map, uint64_t *ba
         : "memory");
 }
 
-// d += a * b on two f32 each.
-__device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, float b0, float b1) {
-    uint64_t a, b, d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(a0), "f"(a1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(b0), "f"(b1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(d0), "f"(d1));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
+// Two f32 in a 64-bit register, for the packed arithmetic.
+using f32x2 = unsigned long long;
+
+__device__ __forceinline__ f32x2 pack(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float2 unpack(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+
+__device__ __forceinline__ void fma2(f32x2 &d, f32x2 a, f32x2 b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b)); }
+
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
 }
 
 struct Smem {
@@ -133,9 +161,9 @@ struct Layout {
     static constexpr int kRing = kWarps * kDepth * kStage;
     static constexpr int kO = kWarps * 8 * NT * DP * 4;
     static constexpr int kQf16 = (SPLIT ? 2 : 1) * 8 * NT * (DP + 8) * 2, kQdigits = 3 * 8 * NT * (DP + 16);
-    static constexpr int kQ = kQf16 > kQdigits ? kQf16 : kQdigits;
+    static constexpr int kQ = ((kQf16 > kQdigits ? kQf16 : kQdigits) + 15) & ~15;  // of the CTA, or of each warp
     static constexpr int kQAt = kRing > kO ? kRing : kO;
-    static constexpr int kBytes = 1024 + kQAt + kQ;
+    static constexpr int bytes(bool solo) { return 1024 + kQAt + (solo ? kWarps : 1) * kQ; }
 };
 
 // A sequence's work: row tiles per head, and block slots of each (an upper
@@ -161,7 +189,7 @@ __device__ __forceinline__ Work work_of(const AttendParams &p, int group, int se
     return w;
 }
 
-template <int DP, int NT, bool SPLIT, bool FP8>
+template <int DP, int NT, bool SPLIT, bool FP8, bool SOLO>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     k_attend(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, AttendParams p) {
     using L = Layout<DP, NT, SPLIT>;
@@ -176,13 +204,27 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     constexpr int kPart = kRows * (DP + 2);   // floats of a part: sums, maxima, sums of weights
     extern __shared__ uint8_t smem_raw[];
     __shared__ Smem sm;
-    __shared__ float s_c[kRows];
+    __shared__ float s_cs[(SOLO ? kWarps : 1) * kRows];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __half *s_q = reinterpret_cast<__half *>(base + L::kQAt);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    __half *s_q = reinterpret_cast<__half *>(base + L::kQAt + (SOLO ? warp * L::kQ : 0));
+    float *s_c = s_cs + (SOLO ? warp * kRows : 0);
+    // an item's warps: all of the CTA's, or this one
+    constexpr int kTeam = SOLO ? 1 : kWarps;
+    const int me = SOLO ? 0 : warp;
+    auto team_sync = [&]() {
+        if (SOLO) __syncwarp();
+        else __syncthreads();
+    };
     const int group = p.q.heads / p.c.heads;
     int8_t *s_d = reinterpret_cast<int8_t *>(s_q);
     uint8_t *ring = base + warp * (kDepth * L::kStage);
+    // where this lane's pieces lie in a K and in a V tile (+ 8 rows: + 8 DP)
+    uint32_t k_at[DP / 64], v_at[2];
+#pragma unroll
+    for (int i = 0; i < DP / 64; i++) k_at[i] = chunk_at<DP>(g, t * (DP / 64) + i);
+#pragma unroll
+    for (int r = 0; r < 2; r++) v_at[r] = chunk_at<DP>(2 * t + r, DP == 128 ? g : g >> 1) + (DP == 128 ? 0 : 8 * (g & 1));
     uint64_t *full = sm.full[warp];
     if (lane == 0) {
         for (int i = 0; i < kDepth; i++) mbar_init(&full[i], 1);
@@ -190,6 +232,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     }
     if (tid == 0) sm.abort = 0;
 
+    int seq = 0, item = 0, off = 0;
+    Work work;
+    long long pos = 0, end = 1, per = 1;
+    if constexpr (!SOLO) {
     // ---- this CTA's share of the block slots: [pos, end) ----
     const int chunk = (p.b.n_seqs + kThreads - 1) / kThreads;  // sequences a thread counts
     const int c_lo = min(tid * chunk, p.b.n_seqs), c_hi = min(c_lo + chunk, p.b.n_seqs);
@@ -212,9 +258,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         if (w < warp) upto += sm.sums[w];
         total += sm.sums[w];
     }
-    const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinBlocks));
-    long long pos = per * blockIdx.x;
-    const long long end = min(total, pos + per);
+    per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinBlocks));
+    pos = per * blockIdx.x;
+    end = min(total, pos + per);
     if (pos >= end) return;
     if (upto - mine <= pos && pos < upto) {
         long long at = upto - mine;
@@ -229,10 +275,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         sm.at = at;
     }
     __syncthreads();
-    int seq = sm.seq;
-    Work work = work_of<kRows>(p, group, seq);
-    int item = static_cast<int>((pos - sm.at) / work.slots);  // of the sequence: head * tiles + tile
-    int off = static_cast<int>(pos - sm.at - static_cast<long long>(item) * work.slots);
+    seq = sm.seq;
+    work = work_of<kRows>(p, group, seq);
+    item = static_cast<int>((pos - sm.at) / work.slots);  // of the sequence: head * tiles + tile
+    off = static_cast<int>(pos - sm.at - static_cast<long long>(item) * work.slots);
+    } else {
+        // items are (sequence, head), dealt out to the warps
+        __syncthreads();
+        pos = blockIdx.x + static_cast<long long>(gridDim.x) * warp;
+        end = static_cast<long long>(p.b.n_seqs) * p.c.heads;
+    }
 
     const int page_mask = (1 << p.c.page_shift) - 1;
     uint32_t phase = 0;  // bit st: parity of the next completion of stage st
@@ -240,14 +292,38 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     bool dead = false;   // a wait ran out
 
     while (pos < end) {
+        if constexpr (SOLO) {
+            seq = static_cast<int>(pos / p.c.heads);
+            item = static_cast<int>(pos - static_cast<long long>(seq) * p.c.heads);
+            work = work_of<kRows>(p, group, seq);
+            if (work.slots == 0) {
+                pos += static_cast<long long>(gridDim.x) * kWarps;
+                continue;
+            }
+        }
         const Span a = work.a;
-        const int n_slots = static_cast<int>(min(static_cast<long long>(work.slots - off), end - pos));
-        const int head = item / work.tiles, tile = item - head * work.tiles;
-        const int rows = a.n * group, r0 = tile * kRows, n_rows = min(kRows, rows - r0), first = a.len - a.n;
-        const int p_lo = first + r0 / group, p_hi = first + (r0 + n_rows - 1) / group;
+        const int n_slots = SOLO ? work.slots : static_cast<int>(min(static_cast<long long>(work.slots - off), end - pos));
+        const int head = SOLO || work.tiles == 1 ? item : item / work.tiles, tile = item - head * work.tiles;
+        const int rows = a.n * group, r0 = SOLO ? 0 : tile * kRows, n_rows = min(kRows, rows - r0), first = a.len - a.n;
+        // row r of the tile is query (skip + r) mod group of the tile's token t0 + (skip + r) / group
+        const int t0 = r0 ? r0 / group : 0, skip = r0 - t0 * group;
+        const float per_group = 1.0f / group;
+        auto tok_of = [&](int r) { return static_cast<int>((skip + r + 0.5f) * per_group); };  // exact: skip + r < 2^17
+        const int p_lo = first + t0, p_hi = p_lo + tok_of(n_rows - 1);
         const Range range = range_of(p_lo, p_hi, p.window, p.sinks, kBlk);
         const int b_lo = off, b_hi = min(range.n, off + n_slots);
 
+        // ---- Q rows into registers ----
+        // (lane l has dimensions 4 l .. 4 l + 3)
+        constexpr int kMine = kRows / kTeam;
+        float4 qx[kMine];
+        const int d4 = 4 * lane;
+#pragma unroll
+        for (int i = 0; i < kMine; i++) {
+            const int r = me + kTeam * i, tok = tok_of(r);
+            const long long at = (a.row0 + t0 + tok) * p.q.ts + (head * group + skip + r - tok * group) * p.q.hs;
+            qx[i] = r < n_rows && d4 < p.c.dim ? load4(p.q, at + d4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
         // ---- this warp's pairs of blocks: b_lo + 2 (warp + 4 i), + 1; lane 2 j + u looks up the
         // page and scales of block u of the (ahead + j)-th pair, half a window before they are used ----
         struct Look {
@@ -256,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         };
         auto look_up = [&](int from) {
             Look k;
-            const int x = b_lo + 2 * (warp + kWarps * (from + (lane >> 1))) + (lane & 1);
+            const int x = b_lo + 2 * (me + kTeam * (from + (lane >> 1))) + (lane & 1);
             const int tok = range.token(x, kBlk);
             k.page = x < b_hi ? page_of(p.c, p.b, seq, tok, p.status) : -1;
             k.sk = k.sv = 0.0f;
@@ -275,21 +351,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             int tok[2];
             float sk[2], sv[2];
         };
-        auto fetch = [&](int stage, int i) {
+        auto start = [&](int stage, int i, Under &u) {
             if (i - ahead == 8) later = look_up(ahead + 16);
             if (i - ahead == 16) {
                 ahead += 16;
                 look = later;
             }
-            Under u;
             int page[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int from = 2 * (i - ahead) + h;
-                page[h] = __shfl_sync(0xffffffffu, look.page, from);
-                u.sk[h] = __shfl_sync(0xffffffffu, look.sk, from);
-                u.sv[h] = __shfl_sync(0xffffffffu, look.sv, from);
-                u.tok[h] = page[h] < 0 ? -1 : range.token(b_lo + 2 * (warp + kWarps * i) + h, kBlk);
+                page[h] = __shfl_sync(0xffffffffu, look.page, 2 * (i - ahead) + h);
+                u.tok[h] = page[h] < 0 ? -1 : range.token(b_lo + 2 * (me + kTeam * i) + h, kBlk);
             }
             const int n = (page[0] >= 0) + (page[1] >= 0);
             if (n && lane == 0) {
@@ -303,28 +375,27 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                         tma_load_3d(&v_map, &full[stage], at + (2 * h + 1) * L::kTile, y, page[h]);
                     }
             }
-            return u;
+        };
+        auto scales = [&](int i, Under &u) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                u.sk[h] = __shfl_sync(0xffffffffu, look.sk, 2 * (i - ahead) + h);
+                u.sv[h] = __shfl_sync(0xffffffffu, look.sv, 2 * (i - ahead) + h);
+            }
         };
 
-        // ---- Q rows into registers, the first blocks under way, Q to f16 ----
-        float qx[kRows / kWarps][DP / 32];
+        Under u0, u1;
+        start(st, 0, u0);
+        start(st ^ 1, 1, u1);
+        scales(0, u0);
+        scales(1, u1);
 #pragma unroll
-        for (int i = 0; i < kRows / kWarps; i++) {
-            const int r = warp + kWarps * i, row = r0 + r, tok = row / group;
-            const long long at = (a.row0 + tok) * p.q.ts + (head * group + row - tok * group) * p.q.hs;
-#pragma unroll
-            for (int e = 0; e < DP / 32; e++) {
-                const int d = lane + 32 * e;
-                qx[i][e] = r < n_rows && d < p.c.dim ? load1(p.q, at + d) : 0.0f;
-            }
-        }
-        Under u0 = fetch(st, 0), u1 = fetch(st ^ 1, 1);
-#pragma unroll
-        for (int i = 0; i < kRows / kWarps; i++) {  // each row by a power of two to below 2
-            const int r = warp + kWarps * i;
+        for (int i = 0; i < kMine; i++) {  // each row by a power of two to below 2
+            const int r = me + kTeam * i;
+            const float x[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
             uint32_t top = 0;
 #pragma unroll
-            for (int e = 0; e < DP / 32; e++) top = max(top, __float_as_uint(qx[i][e]) & 0x7fffffffu);
+            for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
             top = __reduce_max_sync(0xffffffffu, top);
             int e2 = static_cast<int>(top >> 23) - 127;
             e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
@@ -334,24 +405,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                 if (!FP8) c = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : c * 0x1p-21f;
                 s_c[r] = c;
             }
-#pragma unroll
-            for (int e = 0; e < DP / 32; e++) {
-                const int d = lane + 32 * e;
-                const float y = qx[i][e] * down;
-                if (FP8) {
-                    const __half h = __float2half_rn(y);
-                    s_q[r * kQs + d] = h;
-                    if (SPLIT) s_q[(kRows + r) * kQs + d] = __float2half_rn(y - __half2float(h));
-                } else {  // |y| < 2: 23 bits, digits of the sum 65536 d2 + 256 d1 + d0
-                    const int v = __float2int_rn(y * 0x1p21f);
-                    const int d0 = static_cast<int8_t>(v), v1 = (v - d0) >> 8, d1 = static_cast<int8_t>(v1);
-                    s_d[r * kQd + d] = static_cast<int8_t>(d0);
-                    s_d[(kRows + r) * kQd + d] = static_cast<int8_t>(d1);
-                    s_d[(2 * kRows + r) * kQd + d] = static_cast<int8_t>((v1 - d1) >> 8);
+            if (d4 >= DP) continue;
+            if (FP8) {
+                const uint2 h = make_uint2(half2_bits(x[0] * down, x[1] * down), half2_bits(x[2] * down, x[3] * down));
+                *reinterpret_cast<uint2 *>(s_q + r * kQs + d4) = h;
+                if (SPLIT) {
+                    const float2 h0 = half2_floats(h.x), h1 = half2_floats(h.y);
+                    *reinterpret_cast<uint2 *>(s_q + (kRows + r) * kQs + d4) =
+                        make_uint2(half2_bits(x[0] * down - h0.x, x[1] * down - h0.y), half2_bits(x[2] * down - h1.x, x[3] * down - h1.y));
                 }
+            } else {  // |x down| < 2: 23 bits, digits of the sum 65536 d2 + 256 d1 + d0
+                uint32_t digit[3] = {0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int v = __float2int_rn(x[e] * down * 0x1p21f);
+                    const int d0 = static_cast<int8_t>(v), v1 = (v - d0) >> 8, d1 = static_cast<int8_t>(v1), d2 = (v1 - d1) >> 8;
+                    digit[0] |= (d0 & 0xff) << (8 * e);
+                    digit[1] |= (d1 & 0xff) << (8 * e);
+                    digit[2] |= (d2 & 0xff) << (8 * e);
+                }
+#pragma unroll
+                for (int d = 0; d < 3; d++) *reinterpret_cast<uint32_t *>(s_d + (d * kRows + r) * kQd + d4) = digit[d];
             }
         }
-        __syncthreads();
+        team_sync();
 
         float c_row[NT][2];
         int top_key[NT][2], low_key[NT][2];
@@ -361,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             for (int e = 0; e < 2; e++) {
                 const int r = 8 * n + 2 * t + e;
                 c_row[n][e] = s_c[r];
-                top_key[n][e] = r < n_rows ? first + (r0 + r) / group : -1;
+                top_key[n][e] = r < n_rows ? p_lo + tok_of(r) : -1;
                 low_key[n][e] = p.window ? top_key[n][e] - p.window + 1 : 0;
             }
         auto q_frag = [&](int n, int step, int part) {  // part: low half of SPLIT's f16, or the digit
@@ -376,13 +453,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                 for (int d = 0; d < kDigits; d++) qf[kQRegs ? s : 0][d] = q_frag(0, s, d);
         }
 
-        float o[NT][kMt][4], m[NT][2], l[NT][2];
+        // o[n][j]: rows 2t and 2t + 1 of dimension (DP / 8) g + 2 j, then of the next one
+        f32x2 o[NT][kMt][2];
+        float m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
             for (int j = 0; j < kMt; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[n][j][e] = 0.0f;
+                o[n][j][0] = o[n][j][1] = 0;
             m[n][0] = m[n][1] = -INFINITY;
             l[n][0] = l[n][1] = 0.0f;
         }
@@ -394,17 +472,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                 return;
             }
             phase ^= 1u << stage;
-            const uint8_t *tiles = ring + stage * L::kStage;
+            const uint32_t tiles = smem_u32(ring) + stage * L::kStage;
             // ---- S^T = K . Q^T ----
             float sc[2][NT][4];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const uint8_t *kt = tiles + 2 * u * L::kTile;
+                const uint32_t kt = tiles + 2 * u * L::kTile;
                 uint32_t w0[DP / 16], w1[DP / 16];  // tokens g and g + 8, dimensions (DP / 4) t ...
 #pragma unroll
                 for (int i = 0; i < DP / 64; i++) {
-                    const uint4 k0 = *reinterpret_cast<const uint4 *>(chunk_of<DP>(kt, g, t * (DP / 64) + i));
-                    const uint4 k1 = *reinterpret_cast<const uint4 *>(chunk_of<DP>(kt, g + 8, t * (DP / 64) + i));
+                    const uint4 k0 = lds128(kt + k_at[i]), k1 = lds128(kt + k_at[i] + 8 * DP);
                     w0[4 * i] = k0.x, w0[4 * i + 1] = k0.y, w0[4 * i + 2] = k0.z, w0[4 * i + 3] = k0.w;
                     w1[4 * i] = k1.x, w1[4 * i + 1] = k1.y, w1[4 * i + 2] = k1.z, w1[4 * i + 3] = k1.w;
                 }
@@ -424,10 +501,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                         for (int n = 0; n < NT; n++) {
                             float(&acc)[4] = i & 1 ? odd[n] : sc[u][n];
                             const uint2 b = kQRegs ? qf[kQRegs ? i : 0][0] : q_frag(n, i, 0);
-                            mma_f16(acc, f, b.x, b.y);
+                            mma_f16(acc, f, b.x, b.y, acc);
                             if (SPLIT) {
                                 const uint2 low = q_frag(n, i, 1);
-                                mma_f16(acc, f, low.x, low.y);
+                                mma_f16(acc, f, low.x, low.y, acc);
                             }
                         }
                     }
@@ -494,22 +571,25 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             }
             if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int n = 0; n < NT; n++) {
+                    float keep[2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         float x = fmaxf(fmaxf(sc[0][n][e], sc[0][n][e + 2]), fmaxf(sc[1][n][e], sc[1][n][e + 2]));
 #pragma unroll
                         for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
                         x = fmaxf(x, m[n][e]);
-                        const float keep = m[n][e] == -INFINITY ? 0.0f : exp2f(m[n][e] - x);
+                        keep[e] = m[n][e] == -INFINITY ? 0.0f : exp2f(m[n][e] - x);
                         m[n][e] = x;
-                        l[n][e] *= keep;
-#pragma unroll
-                        for (int j = 0; j < kMt; j++) {
-                            o[n][j][e] *= keep;
-                            o[n][j][e + 2] *= keep;
-                        }
+                        l[n][e] *= keep[e];
                     }
+                    const f32x2 k2 = pack(keep[0], keep[1]);
+#pragma unroll
+                    for (int j = 0; j < kMt; j++) {
+                        o[n][j][0] = mul2(o[n][j][0], k2);
+                        o[n][j][1] = mul2(o[n][j][1], k2);
+                    }
+                }
             }
             uint32_t pb[2][NT][2], pl[2][SPLIT ? NT : 1][2];
 #pragma unroll
@@ -539,31 +619,31 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             // error of 2^-23 of 1152 sum(P), about 1e-5 of a typical block's).
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const uint8_t *vt = tiles + (2 * u + 1) * L::kTile;
-                float zero[NT][4], w[NT][2];
+                const uint32_t vt = tiles + (2 * u + 1) * L::kTile;
+                float zero[NT][4];
+                f32x2 w[NT];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) zero[n][e] = 0.0f;
                     const uint32_t minus[4] = {0xe480e480u, 0xe480e480u, 0xe480e480u, 0xe480e480u};
-                    if (kBiased) mma_f16(zero[n], minus, pb[u][n][0], pb[u][n][1]);
-#pragma unroll
-                    for (int e = 0; e < 2; e++) w[n][e] = sees[u][n][e] ? s.sv[u] : 0.0f;
+                    if (kBiased) mma_f16(zero[n], minus, pb[u][n][0], pb[u][n][1], zero[n]);
+                    w[n] = pack(sees[u][n][0] ? s.sv[u] : 0.0f, sees[u][n][1] ? s.sv[u] : 0.0f);
                 }
                 // (an E4M3 NaN in memory past the sequence must not meet a weight of 0)
                 const int seen = whole[u] || !FP8 ? kBlk : s.tok[u] < 0 ? 0 : p_hi + 1 - s.tok[u];
                 uint32_t v[4][DP / 32];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9, dimensions (DP / 8) g ...
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int tok = 2 * t + (r & 1) + 8 * (r >> 1);
+                    const uint32_t at = vt + v_at[r & 1] + (r >> 1) * 8 * DP;
                     if (DP == 128) {
-                        const uint4 x = *reinterpret_cast<const uint4 *>(chunk_of<DP>(vt, tok, g));
+                        const uint4 x = lds128(at);
                         v[r][0] = x.x, v[r][1] = x.y, v[r][DP / 32 - 2] = x.z, v[r][DP / 32 - 1] = x.w;
                     } else {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(chunk_of<DP>(vt, tok, g >> 1) + 8 * (g & 1));
+                        const uint2 x = lds64(at);
                         v[r][0] = x.x, v[r][1] = x.y;
                     }
-                    if (FP8 && tok >= seen) {
+                    if (FP8 && 2 * t + (r & 1) + 8 * (r >> 1) >= seen) {
 #pragma unroll
                         for (int i = 0; i < DP / 32; i++) v[r][i] = 0;
                     }
@@ -578,31 +658,31 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                         const int j = 2 * i + half;
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            float x[4] = {zero[n][0], zero[n][1], zero[n][2], zero[n][3]};
-                            mma_f16(x, f, pb[u][n][0], pb[u][n][1]);
-                            if (SPLIT) mma_f16(x, f, pl[u][SPLIT ? n : 0][0], pl[u][SPLIT ? n : 0][1]);
-                            fma2(o[n][j][0], o[n][j][1], x[0], x[1], w[n][0], w[n][1]);
-                            fma2(o[n][j][2], o[n][j][3], x[2], x[3], w[n][0], w[n][1]);
+                            float x[4];
+                            mma_f16(x, f, pb[u][n][0], pb[u][n][1], zero[n]);
+                            if (SPLIT) mma_f16(x, f, pl[u][SPLIT ? n : 0][0], pl[u][SPLIT ? n : 0][1], x);
+                            fma2(o[n][j][0], pack(x[0], x[1]), w[n]);
+                            fma2(o[n][j][1], pack(x[2], x[3]), w[n]);
                         }
                     }
                 }
             }
         };
 
-        const int n_pairs = (b_hi - b_lo + 1) / 2, n_steps = warp < n_pairs ? (n_pairs - warp + kWarps - 1) / kWarps : 0;
+        const int n_pairs = (b_hi - b_lo + 1) / 2, n_steps = me < n_pairs ? (n_pairs - me + kTeam - 1) / kTeam : 0;
 #pragma unroll 1
         for (int i = 0; i < n_steps; i++) {
             use(st, u0);
             __syncwarp();  // every lane has read the stage
             u0 = u1;
-            u1 = fetch(st, i + kDepth);
+            start(st, i + kDepth, u1);
+            scales(i + kDepth, u1);
             st ^= 1;
         }
         if (dead) {  // give the loads in flight their time before the memory goes to others
             for (int x = 0; x < kDepth; x++) mbar_try_wait(&full[x], (phase >> x) & 1);
         }
 
-        // ---- the warps' sums, in order ----
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -610,21 +690,61 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
                 if (m[n][e] == -INFINITY && l[n][e] != 0.0f) m[n][e] = INFINITY;  // only NaN scores: the row is NaN
-                if (g == 0) {
+            }
+        // four values of row r of the tile
+        auto put = [&](int r, int d, float4 v) {
+            const int tok = tok_of(r);
+            const long long at = (a.row0 + t0 + tok) * p.out.ts + (head * group + skip + r - tok * group) * p.out.hs + d;
+            if (d >= p.c.dim) return;
+            if (p.out.vec) {
+                store4(p.out, at, v);
+            } else {
+                store1(p.out, at, v.x);
+                store1(p.out, at + 1, v.y);
+                store1(p.out, at + 2, v.z);
+                store1(p.out, at + 3, v.w);
+            }
+        };
+        if constexpr (SOLO) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int r = 8 * n + 2 * t + e;
+                    if (r >= n_rows) continue;
+                    const float inv = m[n][e] == -INFINITY ? 0.0f : 1.0f / l[n][e];
+#pragma unroll
+                    for (int j = 0; j < kMt; j += 2) {
+                        const float2 a0 = unpack(o[n][j][0]), a1 = unpack(o[n][j][1]), a2 = unpack(o[n][j + 1][0]), a3 = unpack(o[n][j + 1][1]);
+                        put(r, g * (DP / 8) + 2 * j,
+                            e ? make_float4(a0.y * inv, a1.y * inv, a2.y * inv, a3.y * inv)
+                              : make_float4(a0.x * inv, a1.x * inv, a2.x * inv, a3.x * inv));
+                    }
+                }
+            pos += static_cast<long long>(gridDim.x) * kWarps;
+            __syncwarp();  // Q and the row factors have been read
+        } else {
+        // ---- the warps' sums, in order ----
+        if (g == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
                     sm.m[warp][8 * n + 2 * t + e] = m[n][e];
                     sm.l[warp][8 * n + 2 * t + e] = l[n][e];
                 }
-            }
+        }
         __syncthreads();  // the rings are no longer read: the sums go over them
         float *s_o = reinterpret_cast<float *>(base) + warp * kRows * DP;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int j = 0; j < kMt; j += 2)
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                    *reinterpret_cast<float4 *>(s_o + (8 * n + 2 * t + e) * DP + g * (DP / 8) + 2 * j) =
-                        make_float4(o[n][j][e], o[n][j][e + 2], o[n][j + 1][e], o[n][j + 1][e + 2]);
+            for (int j = 0; j < kMt; j += 2) {
+                const float2 a0 = unpack(o[n][j][0]), a1 = unpack(o[n][j][1]), a2 = unpack(o[n][j + 1][0]), a3 = unpack(o[n][j + 1][1]);
+                float4 *at = reinterpret_cast<float4 *>(s_o + (8 * n + 2 * t) * DP + g * (DP / 8) + 2 * j);
+                at[0] = make_float4(a0.x, a1.x, a2.x, a3.x);
+                at[DP / 4] = make_float4(a0.y, a1.y, a2.y, a3.y);
+            }
         const bool alone = off == 0 && n_slots == work.slots;
         const long long item_at = pos - off;
         const int c0 = static_cast<int>(item_at / per), c1 = static_cast<int>((item_at + work.slots - 1) / per);
@@ -650,19 +770,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             }
         }
         __syncthreads();
-        auto put = [&](int r, int d, float4 v) {
-            const int row = r0 + r, i = row / group;
-            const long long at = (a.row0 + i) * p.out.ts + (head * group + row - i * group) * p.out.hs + d;
-            if (d >= p.c.dim) return;
-            if (p.out.vec) {
-                store4(p.out, at, v);
-            } else {
-                store1(p.out, at, v.x);
-                store1(p.out, at + 1, v.y);
-                store1(p.out, at + 2, v.z);
-                store1(p.out, at + 3, v.w);
-            }
-        };
         const float *all = reinterpret_cast<const float *>(base);
         for (int x = 4 * tid; x < n_rows * DP; x += 4 * kThreads) {
             const int r = x / DP;
@@ -682,16 +789,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             else *reinterpret_cast<float4 *>(part + x) = v;
         }
         if (!alone) {
-            __threadfence();
             __syncthreads();
             if (tid == 0) {
+                __threadfence();  // the CTA's part is written before it is counted
                 int *count = static_cast<int *>(p.ws) + c0;
                 sm.last = atomicAdd(count, 1) == c1 - c0;
                 if (sm.last) *count = 0;
+                __threadfence();
             }
             __syncthreads();
             if (sm.last) {
-                __threadfence();
                 auto part_of = [&](int c) { return parts + (2 * c + (c == c0 ? 1 : 0)) * static_cast<long long>(kPart); };
                 for (int x = 4 * tid; x < n_rows * DP; x += 4 * kThreads) {
                     const int r = x / DP;
@@ -732,6 +839,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             fence_proxy_async_smem();  // the sums were read and written as plain memory, TMA writes there next
             __syncthreads();
         }
+        }
     }
 }
 
@@ -742,22 +850,39 @@ int tiles_of(const Cache &c, int max_new, int q_heads, bool split_f32) {
     return rows <= 8 ? 1 : rows <= 16 || split_f32 ? 2 : 4;
 }
 
+// Blocks a warp takes in the time that an item's beginning and end cost a CTA.
+constexpr int kItemCost = 10;
+
+template <int DP, int NT, bool SPLIT, bool SOLO>
+cudaError_t launch3(const AttendParams &p, const CUtensorMap &k_map, const CUtensorMap &v_map, long long grid, cudaStream_t s) {
+    constexpr int kBytes = Layout<DP, NT, SPLIT>::bytes(SOLO);
+    auto kernel = p.c.fp8 ? k_attend<DP, NT, SPLIT, true, SOLO> : k_attend<DP, NT, SPLIT, false, SOLO>;
+    static SmemOptIn opt_in[2];
+    const cudaError_t e = opt_in[p.c.fp8].set(reinterpret_cast<const void *>(kernel), kBytes);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)grid, kThreads, kBytes, s>>>(k_map, v_map, p);
+    return cudaGetLastError();
+}
+
 template <int DP, int NT, bool SPLIT>
 cudaError_t launch2(const AttendParams &p, int sms, cudaStream_t s) {
-    constexpr int kBytes = Layout<DP, NT, SPLIT>::kBytes;
     CUtensorMap k_map, v_map;
     if (!codes_map(&k_map, p.c, p.c.k, DP, kBlk) || !codes_map(&v_map, p.c, p.c.v, DP, kBlk)) return cudaErrorInvalidValue;
-    auto kernel = p.c.fp8 ? k_attend<DP, NT, SPLIT, true> : k_attend<DP, NT, SPLIT, false>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-    if (e != cudaSuccess) return e;
     // one wave; fewer CTAs when there are not kMinBlocks for each
-    const long long rows = (long long)p.b.max_new * (p.q.heads / p.c.heads);
-    const long long items = (long long)p.b.n_seqs * p.c.heads * ((rows + 8 * NT - 1) / (8 * NT));
-    const long long blocks = p.b.max_len / kBlk + 2;
+    const long long rows = (long long)p.b.max_new * (p.q.heads / p.c.heads), tiles = (rows + 8 * NT - 1) / (8 * NT);
+    const long long items = (long long)p.b.n_seqs * p.c.heads * tiles;
+    long long seen = p.b.max_len;
+    if (p.window) seen = std::min<long long>(seen, (long long)p.window + p.sinks + p.b.max_new + kBlk);
+    const long long blocks = seen / kBlk + 2, wave = (long long)sms * ctas_per_sm<NT, SPLIT>();
+    if constexpr (NT == 1) {
+        // whole items to warps, when the longest would be done before an even
+        // division over CTAs, which pays for the beginning and end of each part
+        const long long solo = (items + kWarps * wave - 1) / (kWarps * wave) * blocks;
+        const long long even = items * blocks / (kWarps * wave) + kItemCost * (items / wave + 2);
+        if (solo <= even) return launch3<DP, NT, SPLIT, true>(p, k_map, v_map, std::min(wave, items), s);
+    }
     const long long most = std::min<long long>(items * ((blocks + kMinBlocks - 1) / kMinBlocks), kCounters);
-    const int grid = (int)std::min<long long>((long long)sms * ctas_per_sm<NT, SPLIT>(), most);
-    kernel<<<grid, kThreads, kBytes, s>>>(k_map, v_map, p);
-    return cudaGetLastError();
+    return launch3<DP, NT, SPLIT, false>(p, k_map, v_map, std::min(wave, most), s);
 }
 
 template <int DP>

@@ -3,6 +3,8 @@
 // helpers that their kernels share.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ditch {
@@ -85,6 +87,21 @@ size_t attend_workspace(const Cache &c, const Batch &b, int q_heads, int sms);
 cudaError_t attend(const AttendParams &p, int sms, cudaStream_t s);
 cudaError_t window_attention(const WindowParams &p, int sms, cudaStream_t s);
 
+// Raises a kernel's dynamic shared memory limit on the current device, once
+// for each device.
+struct SmemOptIn {
+    std::atomic<uint64_t> done{0};
+    cudaError_t set(const void *kernel, int bytes) {
+        int d = 0;
+        cudaError_t e = cudaGetDevice(&d);
+        if (e != cudaSuccess || d > 63 || (done.load(std::memory_order_acquire) >> d & 1) == 0) {
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (e == cudaSuccess && d <= 63) done.fetch_or(1ull << d, std::memory_order_release);
+        }
+        return e;
+    }
+};
+
 // ---- a sequence of a batch ---------------------------------------------------
 // Rows [row0, row0 + n) of the call are the last n of `len` tokens.
 struct Span {
@@ -142,6 +159,18 @@ __device__ __forceinline__ void store1(const Rows &r, long long at, float v) {
     if (r.dtype == kF32) static_cast<float *>(r.p)[at] = v;
     else if (r.dtype == kBf16) static_cast<uint16_t *>(r.p)[at] = f32_to_bf16_bits(v);
     else static_cast<__half *>(r.p)[at] = __float2half_rn(v);
+}
+
+// Four values of a row, at a multiple of four.
+__device__ __forceinline__ float4 load4(const Rows &r, long long at) {
+    if (!r.vec) return make_float4(load1(r, at), load1(r, at + 1), load1(r, at + 2), load1(r, at + 3));
+    if (r.dtype == kF32) return *reinterpret_cast<const float4 *>(static_cast<const float *>(r.p) + at);
+    const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(r.p) + at);
+    if (r.dtype == kBf16)
+        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                           __uint_as_float(u.y & 0xffff0000u));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+    return make_float4(a.x, a.y, b.x, b.y);
 }
 
 // Four values to a 16-byte aligned row, at a multiple of four.
