@@ -845,9 +845,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
 
 // Tiles of 8 rows per CTA. More rows than a CTA takes become row tiles that
 // each read the cache.
-int tiles_of(const Cache &c, int max_new, int q_heads, bool split_f32) {
+int tiles_of(const Cache &c, int max_new, int q_heads) {
     const long long rows = (long long)max_new * (q_heads / c.heads);
-    return rows <= 8 ? 1 : rows <= 16 || split_f32 ? 2 : 4;
+    return rows <= 8 ? 1 : 2;
 }
 
 // Blocks a warp takes in the time that an item's beginning and end cost a CTA.
@@ -888,24 +888,30 @@ cudaError_t launch2(const AttendParams &p, int sms, cudaStream_t s) {
 template <int DP>
 cudaError_t launch1(const AttendParams &p, int nt, bool split_f32, int sms, cudaStream_t s) {
     if (split_f32) return nt == 1 ? launch2<DP, 1, true>(p, sms, s) : launch2<DP, 2, true>(p, sms, s);
-    return nt == 1 ? launch2<DP, 1, false>(p, sms, s) : nt == 2 ? launch2<DP, 2, false>(p, sms, s) : launch2<DP, 4, false>(p, sms, s);
+    return nt == 1 ? launch2<DP, 1, false>(p, sms, s) : launch2<DP, 2, false>(p, sms, s);
 }
 
 }  // namespace
 
 size_t attend_workspace(const Cache &c, const Batch &b, int q_heads, int sms) {
-    size_t floats = 0;
-    for (bool split_f32 : {false, true}) {
-        const int nt = tiles_of(c, b.max_new, q_heads, split_f32);
-        const size_t ctas = std::min<size_t>((size_t)sms * (nt == 1 ? ctas_per_sm<1, false>() : ctas_per_sm<2, false>()), kCounters);
-        floats = std::max(floats, ctas * 2 * (8 * nt) * ((c.dim <= 64 ? 64 : 128) + 2));
-    }
+    const int nt = tiles_of(c, b.max_new, q_heads);
+    const size_t ctas = std::min<size_t>((size_t)sms * (nt == 1 ? ctas_per_sm<1, false>() : ctas_per_sm<2, false>()), kCounters);
+    const size_t floats = ctas * 2 * (8 * nt) * ((c.dim <= 64 ? 64 : 128) + 2);
     return kCounters * sizeof(int) + floats * sizeof(float);
 }
 
 cudaError_t attend(const AttendParams &p, int sms, cudaStream_t s) {
     const bool split_f32 = p.out.dtype == kF32;
-    const int nt = tiles_of(p.c, p.b.max_new, p.q.heads, split_f32);
+    const int nt = tiles_of(p.c, p.b.max_new, p.q.heads);
+    if (!split_f32 && nt > 1) {
+        // Many rows: a tile of 128 keys takes the tiled kernel about 1.5 us for 256 rows, an SM at a time;
+        // here the GPU takes about 1200 blocks of 16 keys by 16 rows a microsecond, wherever they are.
+        const long long rows = (long long)p.b.max_new * (p.q.heads / p.c.heads);
+        long long seen = p.b.max_len;
+        if (p.window) seen = std::min<long long>(seen, (long long)p.window + p.sinks + p.b.max_new);
+        const double here = (double)p.b.n_seqs * p.c.heads * ((rows + 15) / 16) * (seen / kBlk + 1) / 1200.0;
+        if (rows > 16 && 1.5 * tiled_rounds(p, sms, seen) < here) return attend_tiled(p, s);
+    }
     return p.c.dim <= 64 ? launch1<64>(p, nt, split_f32, sms, s) : launch1<128>(p, nt, split_f32, sms, s);
 }
 

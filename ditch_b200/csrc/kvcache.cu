@@ -130,16 +130,6 @@ __device__ __forceinline__ uint2 encode8(bool fp8, const float (&x)[8], float f)
     return make_uint2(encode4(fp8, x, f), encode4(fp8, x + 4, f));
 }
 
-__device__ __forceinline__ void decode4(bool fp8, uint32_t u, float *x) {
-    if (fp8) {
-        const float2 a = e4m3x2_f32(u & 0xffff), b = e4m3x2_f32(u >> 16);
-        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = static_cast<float>(static_cast<int8_t>(u >> (8 * i)));
-    }
-}
-
 // ---- append --------------------------------------------------------------------------
 // The last sequence whose first slot is at most `slot`. Sequences of any
 // lengths get enough slots for their blocks when sequence s starts at slot

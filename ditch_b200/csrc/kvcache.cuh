@@ -86,6 +86,9 @@ cudaError_t read_back(const ReadParams &p, cudaStream_t s);
 size_t attend_workspace(const Cache &c, const Batch &b, int q_heads, int sms);
 cudaError_t attend(const AttendParams &p, int sms, cudaStream_t s);
 cudaError_t window_attention(const WindowParams &p, int sms, cudaStream_t s);
+// The tiled (tcgen05) form of attend, for many rows; and what it costs.
+cudaError_t attend_tiled(const AttendParams &p, cudaStream_t s);
+double tiled_rounds(const AttendParams &p, int sms, long long seen);
 
 // Raises a kernel's dynamic shared memory limit on the current device, once
 // for each device.
@@ -146,6 +149,18 @@ __device__ __forceinline__ long long code_at(const Cache &c, int page, int head,
 __device__ __forceinline__ long long scale_at(const Cache &c, int page, int head, int t) {
     const int in_page = t & ((1 << c.page_shift) - 1);
     return ((static_cast<long long>(page) * c.heads + head) << (c.page_shift - c.block_shift)) + (in_page >> c.block_shift);
+}
+
+// ---- codes -----------------------------------------------------------------------
+// Four codes' values without their scale.
+__device__ __forceinline__ void decode4(bool fp8, uint32_t u, float *x) {
+    if (fp8) {
+        const float2 a = e4m3x2_f32(u & 0xffff), b = e4m3x2_f32(u >> 16);
+        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = static_cast<float>(static_cast<int8_t>(u >> (8 * i)));
+    }
 }
 
 // ---- rows -----------------------------------------------------------------------

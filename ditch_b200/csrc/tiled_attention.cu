@@ -1,5 +1,6 @@
-// Causal attention with a sliding window and sinks over contiguous f16 / bf16
-// rows, on the fifth-generation tensor cores.
+// Causal attention with a sliding window and sinks on the fifth-generation
+// tensor cores, for many query rows: over contiguous f16 / bf16 rows, and over
+// the paged 8-bit cache.
 //
 // Bound by the tensor cores and, just as much, by the exponentials: a 128 x
 // 128 tile of scores takes 512 cycles of MMA for Q.K^T, 512 for P.V (head
@@ -7,7 +8,8 @@
 // of 128 query rows, whose products and softmax alternate:
 //   warps 0-3, 4-7   softmax of the first and second row tile, a row a thread
 //   warp 8           issues the MMAs (one thread)
-//   warp 9           loads (one thread)
+//   warp 9           loads by TMA (one thread; contiguous rows)
+//   warps 12-15      turn 8-bit codes into f16 operands (the cache)
 // A row tile is all the query heads of one key / value head for as many
 // tokens as fill 128 rows, so both tiles read the same keys and values, and a
 // window or the causal limit cuts as close as a few tokens.
@@ -20,12 +22,18 @@
 // taken in P(j): a row whose maximum has grown by more than 2^kLazy since its
 // sums' reference rescales its part of O in TMEM then; most never do.
 //
+// The cache's codes are f16 operands exactly (int8 and E4M3 fit), laid out in
+// shared memory as TMA would; Q is brought into f16's range by a power of two
+// for each row. A block's scales work on the scores: sk in the factor that
+// multiplies them, sv, as a fraction of the largest in sight, in the exponent
+// of the weight that goes into P (taken out again of the sum of weights).
+//
 // What a row does not see has weight 0 in the product, and 0 times an
 // infinity or NaN is NaN: rows whose result is not finite are computed again
-// from the keys that they do see (recompute_row).
+// from the keys that they do see (compute_row).
 //
-// Rows that TMA cannot take (not 16-byte aligned) go by k_window_rows, one
-// warp for each row.
+// Contiguous rows that TMA cannot take (not 16-byte aligned) go by
+// k_window_rows, one warp for each row.
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -67,57 +75,102 @@ __device__ __forceinline__ int first_key(int p, int window, int sinks) {
     return window && sinks == 0 && p >= window ? p - window + 1 : 0;
 }
 
-// Query row `tok` of head `head`, at position pos of the sequence whose keys
-// begin at row k0.
-__device__ __noinline__ void compute_row(const WindowParams &p, int tok, int head, int pos, int k0, int lane) {
-    const int d = 4 * lane, kvh = head / (p.q.heads / p.k.heads);
+// Where keys and values come from.
+struct Contiguous {
+    Rows k, v;
+    const int32_t *ko;
+    int n_kv, max_kv;
+};
+
+struct Paged {
+    Cache c;
+    Batch b;
+};
+
+struct TiledParams {
+    Rows q, out;
+    const int32_t *qo;
+    int n_seqs, n_q, max_q, kv_heads, dim;
+    float scale;
+    int window, sinks;
+    int *status;
+    Contiguous rows;
+    Paged paged;
+};
+
+// Sequence `seq`: its query rows and keys (k0: its first key's row), none
+// (and the status word set) when the device's numbers leave the host's bounds.
+struct Seq {
+    int q0, nq, k0, nk;
+};
+
+template <bool PAGED>
+__device__ __forceinline__ Seq seq_of(const TiledParams &p, int seq) {
+    Seq s;
+    if (PAGED) {
+        const Span a = span_of(p.paged.b, p.paged.c.page_shift, seq, p.status);
+        s.q0 = a.row0, s.nq = a.n, s.k0 = 0, s.nk = a.len;
+        return s;
+    }
+    s.q0 = __ldg(p.qo + seq);
+    s.k0 = __ldg(p.rows.ko + seq);
+    const int q1 = __ldg(p.qo + seq + 1), k1 = __ldg(p.rows.ko + seq + 1);
+    s.nq = q1 - s.q0;
+    s.nk = k1 - s.k0;
+    if (s.q0 < 0 || q1 > p.n_q || s.nq < 0 || s.nq > p.max_q || s.k0 < 0 || k1 > p.rows.n_kv || s.nk < 0 || s.nk > p.rows.max_kv) {
+        flag(p.status);
+        s.nq = s.nk = 0;
+    }
+    return s;
+}
+
+// Query row `tok` of head `head`, at position pos of sequence `seq`, whose
+// contiguous keys begin at row k0.
+template <bool PAGED>
+__device__ __noinline__ void compute_row(const TiledParams &p, int seq, int tok, int head, int pos, int k0, int lane) {
+    const int d = 4 * lane, kvh = head / (p.q.heads / p.kv_heads);
     float q[4] = {0, 0, 0, 0};
     for (int e = 0; e < 4; e++)
         if (d + e < p.dim) q[e] = load1(p.q, tok * p.q.ts + head * p.q.hs + d + e);
     RowState st;
     for (int j = first_key(pos, p.window, p.sinks); j <= pos; j = next_key(j, pos, p.window, p.sinks)) {
         float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-        for (int e = 0; e < 4; e++)
-            if (d + e < p.dim) {
-                k[e] = load1(p.k, (k0 + j) * p.k.ts + kvh * p.k.hs + d + e);
-                v[e] = load1(p.v, (k0 + j) * p.v.ts + kvh * p.v.hs + d + e);
+        if (PAGED) {
+            const Cache &c = p.paged.c;
+            const int page = page_of(c, p.paged.b, seq, j, p.status);
+            if (page < 0) continue;
+            if (d < p.dim) {
+                const long long at = code_at(c, page, kvh, j) + d, sa = scale_at(c, page, kvh, j);
+                decode4(c.fp8, *reinterpret_cast<const uint32_t *>(c.k + at), k);
+                decode4(c.fp8, *reinterpret_cast<const uint32_t *>(c.v + at), v);
+                for (int e = 0; e < 4; e++) {
+                    k[e] *= c.ks[sa];
+                    v[e] *= c.vs[sa];
+                }
             }
+        } else {
+            for (int e = 0; e < 4; e++)
+                if (d + e < p.dim) {
+                    k[e] = load1(p.rows.k, (k0 + j) * p.rows.k.ts + kvh * p.rows.k.hs + d + e);
+                    v[e] = load1(p.rows.v, (k0 + j) * p.rows.v.ts + kvh * p.rows.v.hs + d + e);
+                }
+        }
         st.key(q, k, v, p.scale * kLog2e);
     }
     for (int e = 0; e < 4; e++)
         if (d + e < p.dim) store1(p.out, tok * p.out.ts + head * p.out.hs + d + e, st.m == -INFINITY && st.sum == 0.0f ? 0.0f : st.o[e] / st.sum);
 }
 
-// Sequence `seq` of the batch: its query and key rows, none (and the status
-// word set) when the device's numbers leave the host's bounds.
-struct Seq {
-    int q0, nq, k0, nk;
-};
-
-__device__ __forceinline__ Seq seq_of(const Ragged &b, int seq, int *status) {
-    Seq s;
-    s.q0 = __ldg(b.qo + seq);
-    s.k0 = __ldg(b.ko + seq);
-    const int q1 = __ldg(b.qo + seq + 1), k1 = __ldg(b.ko + seq + 1);
-    s.nq = q1 - s.q0;
-    s.nk = k1 - s.k0;
-    if (s.q0 < 0 || q1 > b.n_q || s.nq < 0 || s.nq > b.max_q || s.k0 < 0 || k1 > b.n_kv || s.nk < 0 || s.nk > b.max_kv) {
-        flag(status);
-        s.nq = s.nk = 0;
-    }
-    return s;
-}
-
-__global__ void __launch_bounds__(kRowWarps * 32) k_window_rows(WindowParams p) {
+__global__ void __launch_bounds__(kRowWarps * 32) k_window_rows(TiledParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row = static_cast<long long>(blockIdx.x) * kRowWarps + warp;
-    if (row >= static_cast<long long>(p.b.n_q) * p.q.heads) return;
+    if (row >= static_cast<long long>(p.n_q) * p.q.heads) return;
     const int tok = static_cast<int>(row / p.q.heads), head = static_cast<int>(row % p.q.heads);
     int seq = 0;
-    while (seq + 1 < p.b.n_seqs && __ldg(p.b.qo + seq + 1) <= tok) seq++;
-    const Seq s = seq_of(p.b, seq, p.status);
+    while (seq + 1 < p.n_seqs && __ldg(p.qo + seq + 1) <= tok) seq++;
+    const Seq s = seq_of<false>(p, seq);
     if (tok < s.q0 || tok >= s.q0 + s.nq) return;
-    compute_row(p, tok, head, s.nk - s.nq + tok - s.q0, s.k0, lane);
+    compute_row<false>(p, seq, tok, head, s.nk - s.nq + tok - s.q0, s.k0, lane);
 }
 
 // ---- the tiled kernel ------------------------------------------------------------------
@@ -125,7 +178,16 @@ constexpr int kTileRows = 128;  // query rows of a tile: the MMA's M, a TMEM lan
 constexpr int kTileKeys = 128;
 constexpr int kBoxKeys = 64;    // keys of one TMA box
 constexpr int kStages = 2;
-constexpr int kThreads = 320;
+constexpr int kConverters = 128;  // threads that turn codes into operands
+constexpr int kScaleSlots = 4;    // tiles whose blocks' scales are kept
+
+// Threads, and the registers they trade at the start (setmaxnreg): the softmax
+// threads hold a row of 128 scores.
+template <bool PAGED>
+struct Team {
+    static constexpr int kThreads = PAGED ? 512 : 384;
+    static constexpr int kSoftmaxRegs = PAGED ? 192 : 208, kIssueRegs = PAGED ? 40 : 80, kConvertRegs = 88;
+};
 
 template <int DP>
 struct WinLayout {
@@ -136,10 +198,23 @@ struct WinLayout {
 
 struct WinBars {
     uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_full[2], o_full[2], scales_full[kScaleSlots];
+    // per 16 keys of a tile: the factor of scores, log2 of sv / the largest sv, its inverse
+    float sk[kScaleSlots][kTileKeys / 16], lv[kScaleSlots][kTileKeys / 16], iv[kScaleSlots][kTileKeys / 16];
+    uint32_t v_top;  // bits of the largest sv in sight
     uint32_t tmem;
     int abort;
 };
+
+template <int N>
+__device__ __forceinline__ void give_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int N>
+__device__ __forceinline__ void take_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 // Shared-memory descriptor of an MN-major operand with 128-byte swizzle, rows
 // of 64 elements for each k: 8 rows are an atom of 1024 bytes (SBO between
@@ -235,11 +310,38 @@ struct Tiling {
     int heads, toks, chunks;
 };
 
-template <int DP, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
-    k_window(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-             const __grid_constant__ CUtensorMap v_map, WindowParams p, Tiling tl, int pairs) {
+// Sixteen codes (dimensions 16 c ... of key r) as two 16-byte pieces of the
+// f16 operand tile, where TMA would have put them.
+template <int DP, bool FP8>
+__device__ __forceinline__ void put_codes(uint8_t *tile, int r, int c, uint4 u) {
+    uint32_t w[8];
+    const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (FP8) {
+            e4m3_pairs(x[i], w[2 * i], w[2 * i + 1]);
+        } else {
+            const uint32_t b = x[i] ^ 0x80808080u;
+            w[2 * i] = int8_pair(b, 0x4140);
+            w[2 * i + 1] = int8_pair(b, 0x4342);
+        }
+    }
+    uint8_t *row = tile + (c >> 2) * WinLayout<DP>::kHalf + r * 128;
+    const int a = 2 * (c & 3), sw = r & 7;
+    // the two halves' lanes store their pieces in opposite order, so that eight lanes cover all banks
+    const bool flip = c >> 2;
+    const uint4 p0 = make_uint4(w[0], w[1], w[2], w[3]), p1 = make_uint4(w[4], w[5], w[6], w[7]);
+    *reinterpret_cast<uint4 *>(row + (((flip ? a + 1 : a) ^ sw) << 4)) = flip ? p1 : p0;
+    *reinterpret_cast<uint4 *>(row + (((flip ? a : a + 1) ^ sw) << 4)) = flip ? p0 : p1;
+}
+
+// OUT: the type of out (and of contiguous operands); the cache's operands are f16.
+template <int DP, bool BF16, bool PAGED, bool FP8>
+__global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
+    k_tiled(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+            const __grid_constant__ CUtensorMap v_map, TiledParams p, Tiling tl, int pairs) {
     using L = WinLayout<DP>;
+    using T = Team<PAGED>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ WinBars bars;
     // the longest runs of keys first
@@ -247,12 +349,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int x = blockIdx.x;
     const int chunk = x % tl.chunks;
     x /= tl.chunks;
-    const int kvh = x % p.k.heads, seq = x / p.k.heads;
-    const Seq sq = seq_of(p.b, seq, p.status);
+    const int kvh = x % p.kv_heads, seq = x / p.kv_heads;
+    const Seq sq = seq_of<PAGED>(p, seq);
     const int i0 = pair * 2 * tl.toks;  // first token of the pair
     if (i0 >= sq.nq) return;
     const int tiles = i0 + tl.toks < sq.nq ? 2 : 1;
-    const int group = p.q.heads / p.k.heads;
+    const int group = p.q.heads / p.kv_heads;
     const int first = sq.nk - sq.nq;  // position of the sequence's first query
     const int p_lo = first + i0, p_hi = first + min(sq.nq, i0 + 2 * tl.toks) - 1;
     Range range = range_of(max(p_lo, 0), max(p_hi, 0), p.window, p.sinks, kTileKeys);
@@ -265,11 +367,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *s_q = base, *s_k = base + 2 * L::kTile, *s_v = s_k + kStages * L::kTile;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(&bars.q_full, 1);
+        mbar_init(&bars.q_full, PAGED ? tiles * kTileRows : 1);
         for (int i = 0; i < kStages; i++) {
-            mbar_init(&bars.k_full[i], 1);
+            mbar_init(&bars.k_full[i], PAGED ? kConverters : 1);
             mbar_init(&bars.k_empty[i], 1);
-            mbar_init(&bars.v_full[i], 1);
+            mbar_init(&bars.v_full[i], PAGED ? kConverters : 1);
             mbar_init(&bars.v_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -277,6 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.p_full[i], kTileRows);
             mbar_init(&bars.o_full[i], 1);
         }
+        for (int i = 0; i < kScaleSlots; i++) mbar_init(&bars.scales_full[i], kConverters);
+        bars.v_top = 0;
         bars.abort = 0;
         fence_barrier_init();
     }
@@ -291,8 +395,83 @@ __global__ void __launch_bounds__(kThreads, 1)
     int *status = p.status;
     volatile int *abort = &bars.abort;
 
-    if (warp == 9) {
-        if (lane == 0 && n > 0) {
+    if (warp >= 8 && warp < 12) give_registers<T::kIssueRegs>();
+    if (PAGED && warp >= 12) {
+        give_registers<T::kConvertRegs>();
+        if (n > 0) {
+            // ---- codes to operands ----
+            const Cache &c = p.paged.c;
+            const int me = tid - 384;
+            // the largest sv in sight (as bits: a NaN is above all)
+            const int per_tile = kTileKeys >> c.block_shift;
+            uint32_t top = 0;
+            for (int b = me; b < n * per_tile; b += kConverters) {
+                const int key = range.token(b / per_tile, kTileKeys) + ((b % per_tile) << c.block_shift);
+                if (key > p_hi) continue;
+                const int page = page_of(c, p.paged.b, seq, key, p.status);
+                if (page >= 0) top = max(top, __float_as_uint(__ldg(c.vs + scale_at(c, page, kvh, key))) & 0x7fffffffu);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) atomicMax(&bars.v_top, top);
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // the converters
+            const float v_top = __uint_as_float(*reinterpret_cast<volatile uint32_t *>(&bars.v_top));
+            constexpr int kChunks = DP / 16;                             // 16-byte pieces of a key's codes
+            constexpr int kMine = kTileKeys * kChunks / kConverters;     // of a thread, for a tile
+            const int chunk16 = me % kChunks, r0 = me / kChunks;         // its keys are r0 + i * kConverters / kChunks
+            // unit u: K (even) or V (odd) of tile u / 2
+            uint4 buf[2][kMine];
+            auto fetch = [&](int u, uint4(&x)[kMine]) {
+                if (u >= 2 * n) return;
+                const int k0 = range.token(u >> 1, kTileKeys);
+                const uint8_t *codes = u & 1 ? c.v : c.k;
+#pragma unroll
+                for (int i = 0; i < kMine; i++) {
+                    const int key = k0 + r0 + i * (kConverters / kChunks);
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (key <= p_hi && 16 * chunk16 < c.dim) {
+                        const int page = page_of(c, p.paged.b, seq, key, p.status);
+                        if (page >= 0) x[i] = __ldg(reinterpret_cast<const uint4 *>(codes + code_at(c, page, kvh, key) + 16 * chunk16));
+                    }
+                }
+            };
+            auto put = [&](int u, const uint4(&x)[kMine]) {
+                const int j = u >> 1, st = j % kStages;
+                const bool value = u & 1;
+                if (!value && me < kTileKeys / 16) {  // the blocks' scales
+                    const int key = range.token(j, kTileKeys) + 16 * me, slot = j % kScaleSlots;
+                    float sk = 0.0f, sv = 0.0f;
+                    if (key <= p_hi) {
+                        const int page = page_of(c, p.paged.b, seq, key, p.status);
+                        const long long at = page >= 0 ? scale_at(c, page, kvh, key) : 0;
+                        sk = page >= 0 ? __ldg(c.ks + at) : __uint_as_float(0x7fc00000u);
+                        sv = page >= 0 ? __ldg(c.vs + at) : 0.0f;
+                    }
+                    // never 0: a hidden score of -inf stays one, a weight of 0 leaves the sum of weights whole
+                    float ratio = sv / v_top;
+                    if (!(ratio >= 0x1p-40f)) ratio = ratio != ratio && v_top != 0.0f ? ratio : 0x1p-40f;
+                    bars.sk[slot][me] = sk == 0.0f ? 0x1p-100f : sk;
+                    bars.lv[slot][me] = log2f(ratio);
+                    bars.iv[slot][me] = 1.0f / ratio;
+                }
+                if (!value) mbar_arrive(&bars.scales_full[j % kScaleSlots]);
+                if (j >= kStages && !mbar_wait(value ? &bars.v_empty[st] : &bars.k_empty[st], (j / kStages + 1) & 1, abort, status)) return false;
+                uint8_t *dst = (value ? s_v : s_k) + st * L::kTile;
+#pragma unroll
+                for (int i = 0; i < kMine; i++) put_codes<DP, FP8>(dst, r0 + i * (kConverters / kChunks), chunk16, x[i]);
+                fence_proxy_async_smem();
+                mbar_arrive(value ? &bars.v_full[st] : &bars.k_full[st]);
+                return true;
+            };
+            fetch(0, buf[0]);
+            for (int u = 0; u < 2 * n; u += 2) {
+                fetch(u + 1, buf[1]);
+                if (!put(u, buf[0])) break;
+                fetch(u + 2, buf[0]);
+                if (!put(u + 1, buf[1])) break;
+            }
+        }
+    } else if (warp == 9) {
+        if (!PAGED && lane == 0 && n > 0) {
             const int head0 = kvh * group + chunk * tl.heads;
             mbar_arrive_expect_tx(&bars.q_full, tiles * (DP / 64) * tl.heads * tl.toks * 128);
             for (int t = 0; t < tiles; t++)
@@ -318,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 8) {
         if (lane == 0 && n > 0) {
-            constexpr uint32_t kType = BF16 ? 1 : 0;
+            constexpr uint32_t kType = BF16 && !PAGED ? 1 : 0;
             auto qk = [&](int t, int j) {
                 const int st = j % kStages;
                 const uint32_t id = idesc_of(kType, false, keys_of(j));
@@ -363,7 +542,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-    } else if ((warp >> 2) < tiles) {
+    } else if (warp < 8) {
+        take_registers<T::kSoftmaxRegs>();
+        if ((warp >> 2) < tiles) {
         // ---- softmax of tile t: this thread's row ----
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
@@ -373,8 +554,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool valid = tok < tl.toks && i < sq.nq && chunk * tl.heads + head < group;
         // the tile's rows: the tiles of keys that all of them see whole need no masks
         const int t_lo = first + i0 + t * tl.toks, t_hi = min(t_lo + tl.toks, first + sq.nq) - 1;
-        const float c = p.scale * kLog2e;
-        float m = -INFINITY, l = 0.0f;  // m in units of the scores
+        float c = p.scale * kLog2e;
+        if (PAGED && n > 0) {
+            // Q to f16: the row by a power of two to below 2, which c makes good
+            const int h = kvh * group + chunk * tl.heads + head;
+            const long long at = (sq.q0 + i) * p.q.ts + h * p.q.hs;
+            uint32_t top = 0;
+            if (valid)
+                for (int d = 0; d < p.dim; d += 4) {
+                    const float4 x = load4(p.q, at + d);
+                    top = max(max(top, __float_as_uint(x.x) & 0x7fffffffu), __float_as_uint(x.y) & 0x7fffffffu);
+                    top = max(max(top, __float_as_uint(x.z) & 0x7fffffffu), __float_as_uint(x.w) & 0x7fffffffu);
+                }
+            int e2 = static_cast<int>(top >> 23) - 127;
+            e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
+            c *= __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+            uint8_t *dst = s_q + t * L::kTile + row * 128;
+#pragma unroll
+            for (int d = 0; d < DP; d += 8) {
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+                if (valid && d < p.dim) {
+                    x = load4(p.q, at + d);
+                    y = load4(p.q, at + d + 4);
+                }
+                *reinterpret_cast<uint4 *>(dst + (d >> 6) * L::kHalf + ((((d & 63) >> 3) ^ (row & 7)) << 4)) =
+                    make_uint4(pack16<false>(x.x * down, x.y * down), pack16<false>(x.z * down, x.w * down),
+                               pack16<false>(y.x * down, y.y * down), pack16<false>(y.z * down, y.w * down));
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bars.q_full);
+        }
+        float m = -INFINITY, l = 0.0f;  // m: the reference maximum of score * c, in base 2
         bool ok = true;
         for (int j = 0; j < n; j++) {
             if (!mbar_wait(&bars.s_full[t], j & 1, abort, status)) {
@@ -395,15 +606,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int b = 0; b < 128; b++)
                     if (b > hi || (b < lo && b >= sink)) s[b] = 0xff800000u;
             }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float f[8];  // factor of the scores of 16 keys
+            if (PAGED) {
+                if (!mbar_wait(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, abort, status)) {
+                    ok = false;
+                    break;
+                }
 #pragma unroll
-            for (int b = 0; b < 128; b += 8)
+                for (int b = 0; b < 8; b++) f[b] = c * bars.sk[j % kScaleSlots][b];
+            }
+            float mx = -INFINITY;
+            if (PAGED) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(s[b + e]), __uint_as_float(s[b + 4 + e])));
-            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            if (__any_sync(0xffffffffu, (mx - m) * c > kLazy)) {
+                for (int b = 0; b < 8; b++) {
+                    float x = __uint_as_float(s[16 * b]), y = __uint_as_float(s[16 * b + 1]);
+#pragma unroll
+                    for (int e = 2; e < 16; e += 2) {
+                        x = fmaxf(x, __uint_as_float(s[16 * b + e]));
+                        y = fmaxf(y, __uint_as_float(s[16 * b + e + 1]));
+                    }
+                    mx = fmaxf(mx, fmaxf(x, y) * f[b]);
+                }
+            } else {
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int b = 0; b < 128; b += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(s[b + e]), __uint_as_float(s[b + 4 + e])));
+                mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+            }
+            if (__any_sync(0xffffffffu, mx - m > kLazy)) {
                 const float to = fmaxf(m, mx);
-                const float keep = m == -INFINITY ? 0.0f : exp2f((m - to) * c);
+                const float keep = m == -INFINITY ? 0.0f : exp2f(m - to);
                 m = to;
                 l *= keep;
                 if (j > 0) {
@@ -419,18 +653,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            const float ref = m == -INFINITY ? 0.0f : -m * c;
+            const float ref = m == -INFINITY ? 0.0f : -m;
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int b = 0; b < 2; b++) {
                 uint32_t w[32];
 #pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    const float a0 = exp2_sfu(fmaf(__uint_as_float(s[64 * b + 2 * e]), c, ref));
-                    const float a1 = exp2_sfu(fmaf(__uint_as_float(s[64 * b + 2 * e + 1]), c, ref));
-                    sum[(2 * e) & 3] += a0;
-                    sum[(2 * e + 1) & 3] += a1;
-                    w[e] = pack16<BF16>(a0, a1);
+                for (int q = 0; q < 4; q++) {
+                    const int at = 64 * b + 16 * q;
+                    const float fb = PAGED ? f[4 * b + q] : c, rb = PAGED ? ref + bars.lv[j % kScaleSlots][4 * b + q] : ref;
+                    float part[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float a0 = exp2_sfu(fmaf(__uint_as_float(s[at + 2 * e]), fb, rb));
+                        const float a1 = exp2_sfu(fmaf(__uint_as_float(s[at + 2 * e + 1]), fb, rb));
+                        if (PAGED) {
+                            part[0] += a0;
+                            part[1] += a1;
+                        } else {
+                            sum[(2 * e) & 3] += a0;
+                            sum[(2 * e + 1) & 3] += a1;
+                        }
+                        w[8 * q + e] = pack16<BF16 && !PAGED>(a0, a1);
+                    }
+                    if (PAGED) sum[q] = fmaf(part[0] + part[1], bars.iv[j % kScaleSlots][4 * b + q], sum[q]);
                 }
                 tmem_st32(s_at + 32 * b, w);
             }
@@ -445,7 +691,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
         }
         if (ok) {
-            const float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+            float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+            if (PAGED && n > 0) inv *= __uint_as_float(bars.v_top);
             const long long at = (sq.q0 + i) * p.out.ts + (kvh * group + chunk * tl.heads + head) * p.out.hs;
             bool odd = false;  // something is not finite
 #pragma unroll
@@ -465,8 +712,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         odd |= !(fabsf(v0) <= 3.4e38f && fabsf(v1) <= 3.4e38f);
                         w[k] = pack16<BF16>(v0, v1);
                     }
-                    if (valid && b + e < p.dim)
+                    if (valid && b + e < p.dim && p.out.vec)
                         *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out.p) + at + b + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    else if (valid && b + e < p.dim)
+#pragma unroll
+                        for (int k = 0; k < 8; k++) static_cast<uint16_t *>(p.out.p)[at + b + e + k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
                 }
             }
             uint32_t again = __ballot_sync(0xffffffffu, valid && odd);
@@ -474,8 +724,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int from = __ffs(again) - 1;
                 again &= again - 1;
                 const int r_i = __shfl_sync(0xffffffffu, i, from), r_head = __shfl_sync(0xffffffffu, head, from);
-                compute_row(p, sq.q0 + r_i, kvh * group + chunk * tl.heads + r_head, first + r_i, sq.k0, lane);
+                compute_row<PAGED>(p, seq, sq.q0 + r_i, kvh * group + chunk * tl.heads + r_head, first + r_i, sq.k0, lane);
             }
+        }
         }
     }
     tc_fence_before();
@@ -494,37 +745,85 @@ bool rows_map(CUtensorMap *map, const Rows &r, int dim, int rows, int box_heads,
                       strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int DP, bool BF16>
-cudaError_t launch(const WindowParams &p, cudaStream_t s) {
-    const int group = p.q.heads / p.k.heads;
+Tiling tiling_of(int group) {
     Tiling tl;
     tl.chunks = (group + kTileRows - 1) / kTileRows;
     tl.heads = (group + tl.chunks - 1) / tl.chunks;
     tl.toks = kTileRows / tl.heads;
-    CUtensorMap q, k, v;
-    if (!rows_map(&q, p.q, p.dim, p.b.n_q, tl.heads, tl.toks) || !rows_map(&k, p.k, p.dim, p.b.n_kv, 1, kBoxKeys) ||
-        !rows_map(&v, p.v, p.dim, p.b.n_kv, 1, kBoxKeys))
+    return tl;
+}
+
+template <int DP, bool BF16, bool PAGED, bool FP8>
+cudaError_t launch(const TiledParams &p, cudaStream_t s) {
+    const Tiling tl = tiling_of(p.q.heads / p.kv_heads);
+    CUtensorMap q{}, k{}, v{};
+    if (!PAGED && (!rows_map(&q, p.q, p.dim, p.n_q, tl.heads, tl.toks) || !rows_map(&k, p.rows.k, p.dim, p.rows.n_kv, 1, kBoxKeys) ||
+                   !rows_map(&v, p.rows.v, p.dim, p.rows.n_kv, 1, kBoxKeys)))
         return cudaErrorInvalidValue;
     static SmemOptIn opt_in;
-    const cudaError_t e = opt_in.set(reinterpret_cast<const void *>(k_window<DP, BF16>), WinLayout<DP>::kBytes);
+    const cudaError_t e = opt_in.set(reinterpret_cast<const void *>(k_tiled<DP, BF16, PAGED, FP8>), WinLayout<DP>::kBytes);
     if (e != cudaSuccess) return e;
-    const int pairs = (p.b.max_q + 2 * tl.toks - 1) / (2 * tl.toks);
-    const long long nx = (long long)p.b.n_seqs * p.k.heads * tl.chunks;
+    const int pairs = (p.max_q + 2 * tl.toks - 1) / (2 * tl.toks);
+    const long long nx = (long long)p.n_seqs * p.kv_heads * tl.chunks;
     if (pairs > 65535 || nx > 0x7fffffffLL) return cudaErrorInvalidValue;
-    k_window<DP, BF16><<<dim3((unsigned)nx, (unsigned)pairs), kThreads, WinLayout<DP>::kBytes, s>>>(q, k, v, p, tl, pairs);
+    k_tiled<DP, BF16, PAGED, FP8><<<dim3((unsigned)nx, (unsigned)pairs), Team<PAGED>::kThreads, WinLayout<DP>::kBytes, s>>>(q, k, v, p, tl, pairs);
     return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t window_attention(const WindowParams &p, int, cudaStream_t s) {
-    if (!p.q.vec || !p.k.vec || !p.v.vec || !p.out.vec || p.b.n_kv == 0) {
-        const long long rows = (long long)p.b.n_q * p.q.heads;
+cudaError_t window_attention(const WindowParams &w, int, cudaStream_t s) {
+    TiledParams p{};
+    p.q = w.q;
+    p.out = w.out;
+    p.qo = w.b.qo;
+    p.n_seqs = w.b.n_seqs;
+    p.n_q = w.b.n_q;
+    p.max_q = w.b.max_q;
+    p.kv_heads = w.k.heads;
+    p.dim = w.dim;
+    p.scale = w.scale;
+    p.window = w.window;
+    p.sinks = w.sinks;
+    p.status = w.status;
+    p.rows = Contiguous{w.k, w.v, w.b.ko, w.b.n_kv, w.b.max_kv};
+    if (!p.q.vec || !w.k.vec || !w.v.vec || !p.out.vec || w.b.n_kv == 0) {
+        const long long rows = (long long)p.n_q * p.q.heads;
         k_window_rows<<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
         return cudaGetLastError();
     }
-    if (p.q.dtype == kBf16) return p.dim <= 64 ? launch<64, true>(p, s) : launch<128, true>(p, s);
-    return p.dim <= 64 ? launch<64, false>(p, s) : launch<128, false>(p, s);
+    if (p.q.dtype == kBf16) return p.dim <= 64 ? launch<64, true, false, false>(p, s) : launch<128, true, false, false>(p, s);
+    return p.dim <= 64 ? launch<64, false, false, false>(p, s) : launch<128, false, false, false>(p, s);
+}
+
+// Rounds of CTAs, one to an SM, times tiles of keys.
+double tiled_rounds(const AttendParams &a, int sms, long long seen) {
+    const Tiling tl = tiling_of(a.q.heads / a.c.heads);
+    const long long items = (long long)a.b.n_seqs * a.c.heads * tl.chunks * ((a.b.max_new + 2 * tl.toks - 1) / (2 * tl.toks));
+    return (double)((items + sms - 1) / sms) * ((seen + kTileKeys - 1) / kTileKeys);
+}
+
+cudaError_t attend_tiled(const AttendParams &a, cudaStream_t s) {
+    TiledParams p{};
+    p.q = a.q;
+    p.out = a.out;
+    p.n_seqs = a.b.n_seqs;
+    p.n_q = a.b.n_tokens;
+    p.max_q = a.b.max_new;
+    p.kv_heads = a.c.heads;
+    p.dim = a.c.dim;
+    p.scale = a.scale;
+    p.window = a.window;
+    p.sinks = a.sinks;
+    p.status = a.status;
+    p.paged = Paged{a.c, a.b};
+    const bool bf16 = a.out.dtype == kBf16;
+    if (p.dim <= 64) {
+        if (a.c.fp8) return bf16 ? launch<64, true, true, true>(p, s) : launch<64, false, true, true>(p, s);
+        return bf16 ? launch<64, true, true, false>(p, s) : launch<64, false, true, false>(p, s);
+    }
+    if (a.c.fp8) return bf16 ? launch<128, true, true, true>(p, s) : launch<128, false, true, true>(p, s);
+    return bf16 ? launch<128, true, true, false>(p, s) : launch<128, false, true, false>(p, s);
 }
 
 }  // namespace kv
