@@ -8,7 +8,8 @@
 // of 128 query rows, whose products and softmax alternate:
 //   warps 0-3, 4-7   softmax of the first and second row tile, a row a thread
 //   warp 8           issues the MMAs (one thread)
-//   warp 9           loads by TMA (one thread; contiguous rows)
+//   warp 9           loads by TMA (contiguous rows), or looks up the pages and
+//                    scales of the tiles to come (the cache)
 //   warps 12-15      turn 8-bit codes into f16 operands (the cache)
 // A row tile is all the query heads of one key / value head for as many
 // tokens as fill 128 rows, so both tiles read the same keys and values, and a
@@ -179,14 +180,14 @@ constexpr int kTileKeys = 128;
 constexpr int kBoxKeys = 64;    // keys of one TMA box
 constexpr int kStages = 2;
 constexpr int kConverters = 128;  // threads that turn codes into operands
-constexpr int kScaleSlots = 4;    // tiles whose blocks' scales are kept
+constexpr int kScaleSlots = 4;    // tiles whose pages and scales are known at a time
 
 // Threads, and the registers they trade at the start (setmaxnreg): the softmax
 // threads hold a row of 128 scores.
 template <bool PAGED>
 struct Team {
     static constexpr int kThreads = PAGED ? 512 : 384;
-    static constexpr int kSoftmaxRegs = PAGED ? 192 : 208, kIssueRegs = PAGED ? 40 : 80, kConvertRegs = 88;
+    static constexpr int kSoftmaxRegs = PAGED ? 184 : 208, kIssueRegs = PAGED ? 40 : 80, kConvertRegs = 104;
 };
 
 template <int DP>
@@ -198,8 +199,10 @@ struct WinLayout {
 
 struct WinBars {
     uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t s_full[2], p_full[2], o_full[2], scales_full[kScaleSlots];
+    uint64_t s_full[2], p_full[2], o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
     // per 16 keys of a tile: the factor of scores, log2 of sv / the largest sv, its inverse
+    // and the offset of their codes (-1: none)
+    long long codes[kScaleSlots][kTileKeys / 16];
     float sk[kScaleSlots][kTileKeys / 16], lv[kScaleSlots][kTileKeys / 16], iv[kScaleSlots][kTileKeys / 16];
     uint32_t v_top;  // bits of the largest sv in sight
     uint32_t tmem;
@@ -379,7 +382,10 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
             mbar_init(&bars.p_full[i], kTileRows);
             mbar_init(&bars.o_full[i], 1);
         }
-        for (int i = 0; i < kScaleSlots; i++) mbar_init(&bars.scales_full[i], kConverters);
+        for (int i = 0; i < kScaleSlots; i++) {
+            mbar_init(&bars.scales_full[i], kTileKeys / 16);
+            mbar_init(&bars.scales_empty[i], 1);
+        }
         bars.v_top = 0;
         bars.abort = 0;
         fence_barrier_init();
@@ -402,58 +408,31 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
             // ---- codes to operands ----
             const Cache &c = p.paged.c;
             const int me = tid - 384;
-            // the largest sv in sight (as bits: a NaN is above all)
-            const int per_tile = kTileKeys >> c.block_shift;
-            uint32_t top = 0;
-            for (int b = me; b < n * per_tile; b += kConverters) {
-                const int key = range.token(b / per_tile, kTileKeys) + ((b % per_tile) << c.block_shift);
-                if (key > p_hi) continue;
-                const int page = page_of(c, p.paged.b, seq, key, p.status);
-                if (page >= 0) top = max(top, __float_as_uint(__ldg(c.vs + scale_at(c, page, kvh, key))) & 0x7fffffffu);
-            }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) atomicMax(&bars.v_top, top);
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // the converters
-            const float v_top = __uint_as_float(*reinterpret_cast<volatile uint32_t *>(&bars.v_top));
             constexpr int kChunks = DP / 16;                             // 16-byte pieces of a key's codes
             constexpr int kMine = kTileKeys * kChunks / kConverters;     // of a thread, for a tile
             const int chunk16 = me % kChunks, r0 = me / kChunks;         // its keys are r0 + i * kConverters / kChunks
             // unit u: K (even) or V (odd) of tile u / 2
+            const bool in = 16 * chunk16 < c.dim;
+            bool live = true;
             uint4 buf[2][kMine];
             auto fetch = [&](int u, uint4(&x)[kMine]) {
                 if (u >= 2 * n) return;
-                const int k0 = range.token(u >> 1, kTileKeys);
-                const uint8_t *codes = u & 1 ? c.v : c.k;
+                const int j = u >> 1, slot = j % kScaleSlots;
+                if (!(u & 1) && live) live = mbar_wait(&bars.scales_full[slot], (j / kScaleSlots) & 1, abort, status);
+                if (!live) return;
+                const uint8_t *codes = (u & 1 ? c.v : c.k) + (r0 & 15) * c.dim + 16 * chunk16;
+                const int last = p_hi - range.token(j, kTileKeys) - r0;
 #pragma unroll
                 for (int i = 0; i < kMine; i++) {
-                    const int key = k0 + r0 + i * (kConverters / kChunks);
-                    x[i] = make_uint4(0, 0, 0, 0);
-                    if (key <= p_hi && 16 * chunk16 < c.dim) {
-                        const int page = page_of(c, p.paged.b, seq, key, p.status);
-                        if (page >= 0) x[i] = __ldg(reinterpret_cast<const uint4 *>(codes + code_at(c, page, kvh, key) + 16 * chunk16));
-                    }
+                    const int at = i * (kConverters / kChunks);
+                    const long long off = bars.codes[slot][(r0 + at) >> 4];
+                    x[i] = at <= last && off >= 0 && in ? __ldg(reinterpret_cast<const uint4 *>(codes + off)) : make_uint4(0, 0, 0, 0);
                 }
             };
             auto put = [&](int u, const uint4(&x)[kMine]) {
                 const int j = u >> 1, st = j % kStages;
                 const bool value = u & 1;
-                if (!value && me < kTileKeys / 16) {  // the blocks' scales
-                    const int key = range.token(j, kTileKeys) + 16 * me, slot = j % kScaleSlots;
-                    float sk = 0.0f, sv = 0.0f;
-                    if (key <= p_hi) {
-                        const int page = page_of(c, p.paged.b, seq, key, p.status);
-                        const long long at = page >= 0 ? scale_at(c, page, kvh, key) : 0;
-                        sk = page >= 0 ? __ldg(c.ks + at) : __uint_as_float(0x7fc00000u);
-                        sv = page >= 0 ? __ldg(c.vs + at) : 0.0f;
-                    }
-                    // never 0: a hidden score of -inf stays one, a weight of 0 leaves the sum of weights whole
-                    float ratio = sv / v_top;
-                    if (!(ratio >= 0x1p-40f)) ratio = ratio != ratio && v_top != 0.0f ? ratio : 0x1p-40f;
-                    bars.sk[slot][me] = sk == 0.0f ? 0x1p-100f : sk;
-                    bars.lv[slot][me] = log2f(ratio);
-                    bars.iv[slot][me] = 1.0f / ratio;
-                }
-                if (!value) mbar_arrive(&bars.scales_full[j % kScaleSlots]);
+                if (!live) return false;
                 if (j >= kStages && !mbar_wait(value ? &bars.v_empty[st] : &bars.k_empty[st], (j / kStages + 1) & 1, abort, status)) return false;
                 uint8_t *dst = (value ? s_v : s_k) + st * L::kTile;
 #pragma unroll
@@ -470,8 +449,50 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                 if (!put(u + 1, buf[1])) break;
             }
         }
+    } else if (PAGED && warp == 9) {
+        if (n > 0) {
+            // ---- pages and scales ----
+            const Cache &c = p.paged.c;
+            // the largest sv in sight (as bits: a NaN is above all)
+            const int per_tile = kTileKeys >> c.block_shift;
+            uint32_t top = 0;
+            for (int b = lane; b < n * per_tile; b += 32) {
+                const int key = range.token(b / per_tile, kTileKeys) + ((b % per_tile) << c.block_shift);
+                if (key > p_hi) continue;
+                const int page = page_of(c, p.paged.b, seq, key, p.status);
+                if (page >= 0) top = max(top, __float_as_uint(__ldg(c.vs + scale_at(c, page, kvh, key))) & 0x7fffffffu);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) bars.v_top = top;
+            const float v_top = __uint_as_float(top);
+            if (lane < kTileKeys / 16)
+                for (int j = 0; j < n; j++) {
+                    const int key = range.token(j, kTileKeys) + 16 * lane, slot = j % kScaleSlots;
+                    float sk = 0.0f, sv = 0.0f;
+                    long long codes = -1;
+                    if (key <= p_hi) {
+                        const int page = page_of(c, p.paged.b, seq, key, p.status);
+                        sk = __uint_as_float(0x7fc00000u);  // no page: the row is computed again without it
+                        if (page >= 0) {
+                            const long long at = scale_at(c, page, kvh, key);
+                            codes = code_at(c, page, kvh, key);
+                            sk = __ldg(c.ks + at);
+                            sv = __ldg(c.vs + at);
+                        }
+                    }
+                    // never 0: a hidden score of -inf stays one, a weight of 0 leaves the sum of weights whole
+                    float ratio = sv / v_top;
+                    if (!(ratio >= 0x1p-40f)) ratio = ratio != ratio && v_top != 0.0f ? ratio : 0x1p-40f;
+                    if (j >= kScaleSlots && !mbar_wait(&bars.scales_empty[slot], (j / kScaleSlots + 1) & 1, abort, status)) break;
+                    bars.codes[slot][lane] = codes;
+                    bars.sk[slot][lane] = sk == 0.0f ? 0x1p-100f : sk;
+                    bars.lv[slot][lane] = log2f(ratio);
+                    bars.iv[slot][lane] = 1.0f / ratio;
+                    mbar_arrive(&bars.scales_full[slot]);
+                }
+        }
     } else if (warp == 9) {
-        if (!PAGED && lane == 0 && n > 0) {
+        if (lane == 0 && n > 0) {
             const int head0 = kvh * group + chunk * tl.heads;
             mbar_arrive_expect_tx(&bars.q_full, tiles * (DP / 64) * tl.heads * tl.toks * 128);
             for (int t = 0; t < tiles; t++)
@@ -528,6 +549,7 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                     for (int k = 0; k < steps; k++)
                         tc_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, v + (k * 16 * 128 >> 4), id, (j | k) ? 1u : 0u);
                     if (t == tiles - 1) tc_commit(&bars.v_empty[st]);
+                    if (PAGED && t == tiles - 1) tc_commit(&bars.scales_empty[j % kScaleSlots]);
                     if (j + 1 < n) {
                         if (t == 0) {
                             ok = mbar_wait(&bars.k_full[(j + 1) % kStages], ((j + 1) / kStages) & 1, abort, status);
