@@ -199,7 +199,7 @@ struct WinLayout {
 
 struct WinBars {
     uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t s_full[2], p_full[2], o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
+    uint64_t s_full[2], p_full[2][2], o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
     // per 16 keys of a tile: the factor of scores, log2 of sv / the largest sv, its inverse
     // and the offset of their codes (-1: none)
     long long codes[kScaleSlots][kTileKeys / 16];
@@ -247,6 +247,15 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         : "memory");
 }
 
+// One lane of a converged warp. The issuing warp runs its loop as a whole, so
+// that descriptors stay in uniform registers, and only the MMAs are this
+// lane's: in a loop of one lane every MMA took about 100 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+
 __device__ __forceinline__ void tma_load_rows(const CUtensorMap *map, uint64_t *bar, void *dst, int d, int head, int row) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
@@ -271,15 +280,6 @@ __device__ __forceinline__ void tmem_ld32_start(uint32_t at, uint32_t *r) {
 // ... and the point after which the registers may be used.
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_ld32_ready(uint32_t *r) {
-    asm volatile(""
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]));
-    asm volatile("" : "+r"(r[30]), "+r"(r[31]));
-}
-
 __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t *r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -299,6 +299,66 @@ __device__ __forceinline__ float exp2_sfu(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Two f32 in a 64-bit register, for the packed arithmetic.
+using f32x2 = unsigned long long;
+
+__device__ __forceinline__ f32x2 pair_of(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float2 floats_of(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 2^x of two numbers not above 2^7 on the FMA pipe, for a share of the
+// exponentials, of which the SFU makes only 16 a cycle: x = n + r with n an
+// integer (rounding by adding 1.5 * 2^23), 2^r on [-1/2, 1/2] by the
+// polynomial of degree 4 with the smallest largest relative error (2.6e-6, by
+// iteratively reweighted least squares), n added to the exponent. Numbers
+// below -126 give 2^-126; a NaN gives something that is not finite in 16 bits.
+__device__ __forceinline__ float2 exp2_fma(f32x2 x) {
+    const float2 v = floats_of(x);
+    float lo, hi;
+    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(lo) : "f"(v.x));
+    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(hi) : "f"(v.y));
+    x = pair_of(lo, hi);
+    const f32x2 n = add2(x, pair_of(12582912.0f, 12582912.0f));
+    const f32x2 r = fma2(add2(n, pair_of(-12582912.0f, -12582912.0f)), pair_of(-1.0f, -1.0f), x);
+    f32x2 y = pair_of(0.009570102207362652f, 0.009570102207362652f);
+    y = fma2(y, r, pair_of(0.05591786280274391f, 0.05591786280274391f));
+    y = fma2(y, r, pair_of(0.240247443318367f, 0.240247443318367f));
+    y = fma2(y, r, pair_of(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(y, r, pair_of(0.9999992847442627f, 0.9999992847442627f));
+    const float2 p = floats_of(y), k = floats_of(n);
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(k.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(k.y) << 23)));
+}
+
+// Which of the eight pairs of 16 keys take the FMA pipe.
+constexpr uint32_t kByFma = 0x00;
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -379,7 +439,8 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.s_full[i], 1);
-            mbar_init(&bars.p_full[i], kTileRows);
+            mbar_init(&bars.p_full[i][0], kTileRows);
+            mbar_init(&bars.p_full[i][1], kTileRows);
             mbar_init(&bars.o_full[i], 1);
         }
         for (int i = 0; i < kScaleSlots; i++) {
@@ -517,39 +578,57 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
         loads_done:;
         }
     } else if (warp == 8) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             constexpr uint32_t kType = BF16 && !PAGED ? 1 : 0;
+            const bool leader = elect_one();
+            const uint32_t q_at = smem_u32(s_q), k_at = smem_u32(s_k), v_at = smem_u32(s_v);
             auto qk = [&](int t, int j) {
-                const int st = j % kStages;
                 const uint32_t id = idesc_of(kType, false, keys_of(j));
+                const uint64_t a = sw128_kmajor_desc(q_at + t * L::kTile), b = sw128_kmajor_desc(k_at + (j % kStages) * L::kTile);
+                const uint32_t d = tmem + 128 * t;
+                if (leader) {
 #pragma unroll
-                for (int h = 0; h < DP / 64; h++) {
-                    const uint64_t a = sw128_kmajor_desc(smem_u32(s_q + t * L::kTile + h * L::kHalf));
-                    const uint64_t b = sw128_kmajor_desc(smem_u32(s_k + st * L::kTile + h * L::kHalf));
+                    for (int h = 0; h < DP / 64; h++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) tc_mma_bf16(tmem + 128 * t, a + 2 * k, b + 2 * k, id, (h | k) ? 1u : 0u);
+                        for (int k = 0; k < 4; k++)
+                            tc_mma_bf16(d, a + (h * L::kHalf >> 4) + 2 * k, b + (h * L::kHalf >> 4) + 2 * k, id, (h | k) ? 1u : 0u);
+                    tc_commit(&bars.s_full[t]);
                 }
-                tc_commit(&bars.s_full[t]);
+                __syncwarp();
+            };
+            auto commit = [&](uint64_t *bar) {
+                if (leader) tc_commit(bar);
+                __syncwarp();
             };
             bool ok = mbar_wait(&bars.q_full, 0, abort, status) && mbar_wait(&bars.k_full[0], 0, abort, status);
             if (ok) {
                 tc_fence_after();
                 for (int t = 0; t < tiles; t++) qk(t, 0);
-                tc_commit(&bars.k_empty[0]);
+                commit(&bars.k_empty[0]);
             }
             for (int j = 0; ok && j < n; j++) {
                 const int st = j % kStages, steps = keys_of(j) / 16;
                 for (int t = 0; ok && t < tiles; t++) {
-                    ok = mbar_wait(&bars.p_full[t], j & 1, abort, status);
-                    if (ok && t == 0) ok = mbar_wait(&bars.v_full[st], (j / kStages) & 1, abort, status);
+                    const uint32_t id = idesc_of(kType, true, DP), d = tmem + 256 + 128 * t, a = tmem + 128 * t;
+                    const uint64_t v = sw128_mnmajor_desc(v_at + st * L::kTile, L::kHalf);
+                    for (int half = 0; ok && half < 2; half++) {  // P comes in halves of 64 keys
+                        ok = mbar_wait(&bars.p_full[t][half], j & 1, abort, status);
+                        if (ok && t == 0 && half == 0) ok = mbar_wait(&bars.v_full[st], (j / kStages) & 1, abort, status);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (leader) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                if (4 * half + k < steps)
+                                    tc_mma_ts(d, a + 8 * (4 * half + k), v + (4 * half + k) * (16 * 128 >> 4), id, (j | half | k) ? 1u : 0u);
+                        }
+                        __syncwarp();
+                    }
                     if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t id = idesc_of(kType, true, DP);
-                    const uint64_t v = sw128_mnmajor_desc(smem_u32(s_v + st * L::kTile), L::kHalf);
-                    for (int k = 0; k < steps; k++)
-                        tc_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, v + (k * 16 * 128 >> 4), id, (j | k) ? 1u : 0u);
-                    if (t == tiles - 1) tc_commit(&bars.v_empty[st]);
-                    if (PAGED && t == tiles - 1) tc_commit(&bars.scales_empty[j % kScaleSlots]);
+                    if (t == tiles - 1) {
+                        commit(&bars.v_empty[st]);
+                        if (PAGED) commit(&bars.scales_empty[j % kScaleSlots]);
+                    }
                     if (j + 1 < n) {
                         if (t == 0) {
                             ok = mbar_wait(&bars.k_full[(j + 1) % kStages], ((j + 1) / kStages) & 1, abort, status);
@@ -557,9 +636,9 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                             tc_fence_after();
                         }
                         qk(t, j + 1);
-                        if (t == tiles - 1) tc_commit(&bars.k_empty[(j + 1) % kStages]);
+                        if (t == tiles - 1) commit(&bars.k_empty[(j + 1) % kStages]);
                     } else {
-                        tc_commit(&bars.o_full[t]);
+                        commit(&bars.o_full[t]);
                     }
                 }
             }
@@ -619,8 +698,6 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
 #pragma unroll
             for (int b = 0; b < 4; b++) tmem_ld32_start(s_at + 32 * b, s + 32 * b);
             tmem_ld_wait();
-#pragma unroll
-            for (int b = 0; b < 4; b++) tmem_ld32_ready(s + 32 * b);
             const int k0 = range.token(j, kTileKeys);
             if (k0 + kTileKeys - 1 > t_lo || (p.window && k0 <= t_hi - p.window)) {
                 const int hi = pos - k0, lo = p.window ? hi - p.window + 1 : 0, sink = p.sinks - k0;
@@ -643,10 +720,11 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                 for (int b = 0; b < 8; b++) {
                     float x = __uint_as_float(s[16 * b]), y = __uint_as_float(s[16 * b + 1]);
 #pragma unroll
-                    for (int e = 2; e < 16; e += 2) {
-                        x = fmaxf(x, __uint_as_float(s[16 * b + e]));
-                        y = fmaxf(y, __uint_as_float(s[16 * b + e + 1]));
+                    for (int e = 2; e < 14; e += 4) {
+                        x = max3(x, __uint_as_float(s[16 * b + e]), __uint_as_float(s[16 * b + e + 1]));
+                        y = max3(y, __uint_as_float(s[16 * b + e + 2]), __uint_as_float(s[16 * b + e + 3]));
                     }
+                    x = max3(x, __uint_as_float(s[16 * b + 14]), __uint_as_float(s[16 * b + 15]));
                     mx = fmaxf(mx, fmaxf(x, y) * f[b]);
                 }
             } else {
@@ -654,7 +732,7 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
 #pragma unroll
                 for (int b = 0; b < 128; b += 8)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(s[b + e]), __uint_as_float(s[b + 4 + e])));
+                    for (int e = 0; e < 4; e++) top[e] = max3(top[e], __uint_as_float(s[b + e]), __uint_as_float(s[b + 4 + e]));
                 mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
             }
             if (__any_sync(0xffffffffu, mx - m > kLazy)) {
@@ -668,7 +746,6 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                         uint32_t o[32];
                         tmem_ld32_start(o_at + b, o);
                         tmem_ld_wait();
-                        tmem_ld32_ready(o);
 #pragma unroll
                         for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
                         tmem_st32(o_at + b, o);
@@ -676,36 +753,48 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                 }
             }
             const float ref = m == -INFINITY ? 0.0f : -m;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            f32x2 sum[2] = {0, 0};
+            // by quarters of 32 keys; the first half of P is handed over while the last quarter is made
+            uint32_t w[32];
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                uint32_t w[32];
+            for (int b = 0; b < 4; b++) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int at = 64 * b + 16 * q;
-                    const float fb = PAGED ? f[4 * b + q] : c, rb = PAGED ? ref + bars.lv[j % kScaleSlots][4 * b + q] : ref;
-                    float part[2] = {0.0f, 0.0f};
+                for (int q = 0; q < 2; q++) {
+                    const int at = 32 * b + 16 * q;
+                    const float fb = PAGED ? f[2 * b + q] : c, rb = PAGED ? ref + bars.lv[j % kScaleSlots][2 * b + q] : ref;
+                    const f32x2 f2 = pair_of(fb, fb), r2 = pair_of(rb, rb);
+                    f32x2 part[2] = {0, 0};
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float a0 = exp2_sfu(fmaf(__uint_as_float(s[at + 2 * e]), fb, rb));
-                        const float a1 = exp2_sfu(fmaf(__uint_as_float(s[at + 2 * e + 1]), fb, rb));
-                        if (PAGED) {
-                            part[0] += a0;
-                            part[1] += a1;
+                        const f32x2 x = fma2(pair_of(__uint_as_float(s[at + 2 * e]), __uint_as_float(s[at + 2 * e + 1])), f2, r2);
+                        float2 a;
+                        if (kByFma >> e & 1) {
+                            a = exp2_fma(x);
                         } else {
-                            sum[(2 * e) & 3] += a0;
-                            sum[(2 * e + 1) & 3] += a1;
+                            const float2 v = floats_of(x);
+                            a = make_float2(exp2_sfu(v.x), exp2_sfu(v.y));
                         }
-                        w[8 * q + e] = pack16<BF16 && !PAGED>(a0, a1);
+                        f32x2 &to = PAGED ? part[e & 1] : sum[e & 1];
+                        to = add2(to, pair_of(a.x, a.y));
+                        w[16 * (b & 1) + 8 * q + e] = pack16<BF16 && !PAGED>(a.x, a.y);
                     }
-                    if (PAGED) sum[q] = fmaf(part[0] + part[1], bars.iv[j % kScaleSlots][4 * b + q], sum[q]);
+                    if (PAGED) {
+                        const float iv = bars.iv[j % kScaleSlots][2 * b + q];
+                        sum[q] = fma2(add2(part[0], part[1]), pair_of(iv, iv), sum[q]);
+                    }
                 }
-                tmem_st32(s_at + 32 * b, w);
+                if (b == 2) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&bars.p_full[t][0]);
+                }
+                if (b & 1) tmem_st32(s_at + 16 * (b - 1), w);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const float2 s2 = floats_of(add2(sum[0], sum[1]));
+            l += s2.x + s2.y;
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&bars.p_full[t]);
+            mbar_arrive(&bars.p_full[t][1]);
         }
         // ---- out = O / l ----
         if (ok && n > 0) {
@@ -713,7 +802,7 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
             tc_fence_after();
         }
         if (ok) {
-            float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+            float inv = m == -INFINITY && l == l ? 0.0f : 1.0f / l;  // (hidden weights may be 2^-126)
             if (PAGED && n > 0) inv *= __uint_as_float(bars.v_top);
             const long long at = (sq.q0 + i) * p.out.ts + (kvh * group + chunk * tl.heads + head) * p.out.hs;
             bool odd = false;  // something is not finite
@@ -723,7 +812,6 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                 if (n > 0) {
                     tmem_ld32_start(o_at + b, o);
                     tmem_ld_wait();
-                    tmem_ld32_ready(o);
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
