@@ -904,13 +904,13 @@ cudaError_t attend(const AttendParams &p, int sms, cudaStream_t s) {
     const bool split_f32 = p.out.dtype == kF32;
     const int nt = tiles_of(p.c, p.b.max_new, p.q.heads);
     if (!split_f32 && nt > 1) {
-        // Many rows: a tile of 128 keys takes the tiled kernel about 1.5 us for 256 rows, an SM at a time;
+        // Many rows: a tile of 64 keys takes the tiled kernel about 0.8 us for 256 rows, an SM at a time;
         // here the GPU takes about 1200 blocks of 16 keys by 16 rows a microsecond, wherever they are.
         const long long rows = (long long)p.b.max_new * (p.q.heads / p.c.heads);
         long long seen = p.b.max_len;
         if (p.window) seen = std::min<long long>(seen, (long long)p.window + p.sinks + p.b.max_new);
         const double here = (double)p.b.n_seqs * p.c.heads * ((rows + 15) / 16) * (seen / kBlk + 1) / 1200.0;
-        if (rows > 16 && 1.5 * tiled_rounds(p, sms, seen) < here) return attend_tiled(p, s);
+        if (rows > 16 && 0.8 * tiled_rounds(p, sms, seen) < here) return attend_tiled(p, s);
     }
     return p.c.dim <= 64 ? launch1<64>(p, nt, split_f32, sms, s) : launch1<128>(p, nt, split_f32, sms, s);
 }

@@ -2,26 +2,34 @@
 // tensor cores, for many query rows: over contiguous f16 / bf16 rows, and over
 // the paged 8-bit cache.
 //
-// Bound by the tensor cores and, just as much, by the exponentials: a 128 x
-// 128 tile of scores takes 512 cycles of MMA for Q.K^T, 512 for P.V (head
-// size 128) and 1024 cycles of the SFU. One CTA therefore works on two tiles
-// of 128 query rows, whose products and softmax alternate:
-//   warps 0-3, 4-7   softmax of the first and second row tile, a row a thread
-//   warp 8           issues the MMAs (one thread)
-//   warp 9           loads by TMA (contiguous rows), or looks up the pages and
+// Bound by the tensor cores and, just as much, by the exponentials: 128 x 128
+// scores take 512 cycles of MMA for Q.K^T, 512 for P.V (head size 128) and
+// 1024 cycles of the SFU. Two row tiles of 128 query rows are on an SM, whose
+// products and softmax alternate, in one CTA or in two:
+//   first warps      softmax, four warps a row tile, a row a thread
+//   then one         issues the MMAs
+//   then one         loads by TMA (contiguous rows), or looks up the pages and
 //                    scales of the tiles to come (the cache)
 //   warps 12-15      turn 8-bit codes into f16 operands (the cache)
 // A row tile is all the query heads of one key / value head for as many
-// tokens as fill 128 rows, so both tiles read the same keys and values, and a
-// window or the causal limit cuts as close as a few tokens.
+// tokens as fill 128 rows, so that a window or the causal limit cuts as close
+// as a few tokens, and two tiles of one CTA read the same keys and values.
 //
-// TMEM: S of both tiles (128 columns each), O of both (128 each). P goes back
-// over its S as 16-bit pairs and is the A operand of P.V from there; V is
-// taken as it lies, [token][dimension], as a transposed (MN-major) B operand.
-// The MMAs of one CTA complete in the order of their issue, so S(j + 1) of a
-// tile may be issued right behind P.V(j), and when S(j + 1) is there, O has
-// taken in P(j): a row whose maximum has grown by more than 2^kLazy since its
-// sums' reference rescales its part of O in TMEM then; most never do.
+// TMEM: for each row tile S (128 columns: one tile of 128 keys, or two of 64)
+// and O (128). P goes back over its S as 16-bit pairs and is the A operand of
+// P.V from there; V is taken as it lies, [token][dimension], as a transposed
+// (MN-major) B operand. Three shapes (Shape), by measurement at head size 128:
+//   128 keys, two row tiles a CTA: the least MMA time, for long runs of keys
+//     (8192 tokens, window 4096: 710 us, against 928 us with 64 keys: an MMA
+//     with N = 64 takes the 64 cycles of one with N = 128, for its A operand)
+//   64 keys, two row tiles: S(j + 1) is made while the softmax works on S(j);
+//     for the cache, whose codes then need half the registers on their way
+//     (512 tokens over 1000 to 8000: 238 us against 307 us)
+//   64 keys, one row tile, two CTAs an SM: short runs, where the beginning
+//     and end of a CTA count
+// A row whose maximum has grown by more than 2^kLazy since its sums'
+// reference rescales its part of O in TMEM, once P.V(j - 1) is in; most never
+// do.
 //
 // The cache's codes are f16 operands exactly (int8 and E4M3 fit), laid out in
 // shared memory as TMA would; Q is brought into f16's range by a power of two
@@ -176,34 +184,42 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_window_rows(TiledParams p) {
 
 // ---- the tiled kernel ------------------------------------------------------------------
 constexpr int kTileRows = 128;  // query rows of a tile: the MMA's M, a TMEM lane each
-constexpr int kTileKeys = 128;
-constexpr int kBoxKeys = 64;    // keys of one TMA box
-constexpr int kStages = 2;
+
+// KEYS: of a tile; TILES: row tiles of a CTA.
+template <bool PAGED_, int KEYS_, int TILES_>
+struct Shape {
+    static constexpr bool kPaged = PAGED_;
+    static constexpr int kKeys = KEYS_, kTiles = TILES_;
+    static constexpr int kBuffers = 128 / KEYS_;                       // of S, a row tile
+    static constexpr int kStages = KEYS_ == 128 || TILES_ == 1 ? 2 : 4;  // tiles of K and of V in shared memory
+    // Registers that the softmax warps take from the others at the start (setmaxnreg; 512 threads begin with 128
+    // each, 384 with 168): they hold a row of scores. With 64 keys and no converters, what they begin with is enough.
+    static constexpr bool kTrade = PAGED_ || KEYS_ == 128;
+    static constexpr int kThreads = PAGED_ ? 512 : kTrade ? 384 : 128 * TILES_ + 64;
+    static constexpr int kSoftmaxRegs = PAGED_ ? 160 : 208, kIssueRegs = 80, kConvertRegs = 112;
+    static constexpr int kCtas = TILES_ == 1 ? 2 : 1;                  // an SM
+    static constexpr int kIssuer = 4 * TILES_, kLoader = kIssuer + 1;  // warps
+    static constexpr uint32_t kTmem = 256 * TILES_;
+};
 constexpr int kConverters = 128;  // threads that turn codes into operands
-constexpr int kScaleSlots = 4;    // tiles whose pages and scales are known at a time
+constexpr int kScaleSlots = 8;    // tiles whose pages and scales are known at a time
 
-// Threads, and the registers they trade at the start (setmaxnreg): the softmax
-// threads hold a row of 128 scores.
-template <bool PAGED>
-struct Team {
-    static constexpr int kThreads = PAGED ? 512 : 384;
-    static constexpr int kSoftmaxRegs = PAGED ? 184 : 208, kIssueRegs = PAGED ? 40 : 80, kConvertRegs = 104;
+template <int DP, class S>
+struct Layout {
+    static constexpr int kQHalf = kTileRows * 128, kKHalf = S::kKeys * 128;  // 64 dimensions of a tile's rows
+    static constexpr int kQTile = kQHalf * (DP / 64), kKTile = kKHalf * (DP / 64);
+    static constexpr int kBytes = 1024 + S::kTiles * kQTile + 2 * S::kStages * kKTile;
 };
 
-template <int DP>
-struct WinLayout {
-    static constexpr int kHalf = kTileRows * 128;             // 64 dimensions of 128 rows
-    static constexpr int kTile = kHalf * (DP / 64);           // a tile of Q, K or V
-    static constexpr int kBytes = 1024 + (2 + 2 * kStages) * kTile;
-};
+constexpr int kMostStages = 4, kScaleKeys = 64;  // (the cache's tiles are of 64 keys)
 
-struct WinBars {
-    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t s_full[2], p_full[2][2], o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
+struct Bars {
+    uint64_t q_full, k_full[kMostStages], k_empty[kMostStages], v_full[kMostStages], v_empty[kMostStages];
+    uint64_t s_full[2][2], p_full[2][2], o_done[2], o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
     // per 16 keys of a tile: the factor of scores, log2 of sv / the largest sv, its inverse
     // and the offset of their codes (-1: none)
-    long long codes[kScaleSlots][kTileKeys / 16];
-    float sk[kScaleSlots][kTileKeys / 16], lv[kScaleSlots][kTileKeys / 16], iv[kScaleSlots][kTileKeys / 16];
+    long long codes[kScaleSlots][kScaleKeys / 16];
+    float sk[kScaleSlots][kScaleKeys / 16], lv[kScaleSlots][kScaleKeys / 16], iv[kScaleSlots][kScaleKeys / 16];
     uint32_t v_top;  // bits of the largest sv in sight
     uint32_t tmem;
     int abort;
@@ -292,6 +308,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t *r) {
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16_start(uint32_t at, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float exp2_sfu(float x) {
@@ -375,8 +399,8 @@ struct Tiling {
 
 // Sixteen codes (dimensions 16 c ... of key r) as two 16-byte pieces of the
 // f16 operand tile, where TMA would have put them.
-template <int DP, bool FP8>
-__device__ __forceinline__ void put_codes(uint8_t *tile, int r, int c, uint4 u) {
+template <bool FP8>
+__device__ __forceinline__ void put_codes(uint8_t *tile, int half_bytes, int r, int c, uint4 u) {
     uint32_t w[8];
     const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -389,7 +413,7 @@ __device__ __forceinline__ void put_codes(uint8_t *tile, int r, int c, uint4 u) 
             w[2 * i + 1] = int8_pair(b, 0x4342);
         }
     }
-    uint8_t *row = tile + (c >> 2) * WinLayout<DP>::kHalf + r * 128;
+    uint8_t *row = tile + (c >> 2) * half_bytes + r * 128;
     const int a = 2 * (c & 3), sw = r & 7;
     // the two halves' lanes store their pieces in opposite order, so that eight lanes cover all banks
     const bool flip = c >> 2;
@@ -398,28 +422,38 @@ __device__ __forceinline__ void put_codes(uint8_t *tile, int r, int c, uint4 u) 
     *reinterpret_cast<uint4 *>(row + (((flip ? a : a + 1) ^ sw) << 4)) = flip ? p0 : p1;
 }
 
-// OUT: the type of out (and of contiguous operands); the cache's operands are f16.
-template <int DP, bool BF16, bool PAGED, bool FP8>
-__global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
+// BF16: the type of out (and of contiguous operands); the cache's operands are f16.
+template <int DP, bool BF16, bool FP8, class S>
+__global__ void __launch_bounds__(S::kThreads, S::kCtas)
     k_tiled(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
             const __grid_constant__ CUtensorMap v_map, TiledParams p, Tiling tl, int pairs) {
-    using L = WinLayout<DP>;
-    using T = Team<PAGED>;
+    using L = Layout<DP, S>;
+    constexpr bool PAGED = S::kPaged;
+    constexpr int kTileKeys = S::kKeys, kStages = S::kStages, kBuffers = S::kBuffers;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ WinBars bars;
-    // the longest runs of keys first
-    const int pair = pairs - 1 - blockIdx.y;
-    int x = blockIdx.x;
-    const int chunk = x % tl.chunks;
-    x /= tl.chunks;
-    const int kvh = x % p.kv_heads, seq = x / p.kv_heads;
+    __shared__ Bars bars;
+    // the longest runs of keys first: the longest sequences (where there are few), and their last rows
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int pair = pairs - 1 - blockIdx.x / (tl.chunks * p.kv_heads);
+    int x = blockIdx.x % (tl.chunks * p.kv_heads), seq = blockIdx.y;
+    if (p.n_seqs <= 32 && p.n_seqs > 1) {
+        int len = -1;
+        if (lane < p.n_seqs) len = PAGED ? __ldg(p.paged.b.lens + lane) : __ldg(p.rows.ko + lane + 1) - __ldg(p.rows.ko + lane);
+        int before = 0;
+        for (int i = 0; i < p.n_seqs; i++) {
+            const int other = __shfl_sync(0xffffffffu, len, i);
+            before += other > len || (other == len && i < lane);
+        }
+        seq = __ffs(__ballot_sync(0xffffffffu, lane < p.n_seqs && before == static_cast<int>(blockIdx.y))) - 1;
+    }
+    const int chunk = x % tl.chunks, kvh = x / tl.chunks;
     const Seq sq = seq_of<PAGED>(p, seq);
-    const int i0 = pair * 2 * tl.toks;  // first token of the pair
+    const int i0 = pair * S::kTiles * tl.toks;  // first token of the CTA's
     if (i0 >= sq.nq) return;
-    const int tiles = i0 + tl.toks < sq.nq ? 2 : 1;
+    const int tiles = S::kTiles == 2 && i0 + tl.toks < sq.nq ? 2 : 1;
     const int group = p.q.heads / p.kv_heads;
     const int first = sq.nk - sq.nq;  // position of the sequence's first query
-    const int p_lo = first + i0, p_hi = first + min(sq.nq, i0 + 2 * tl.toks) - 1;
+    const int p_lo = first + i0, p_hi = first + min(sq.nq, i0 + S::kTiles * tl.toks) - 1;
     Range range = range_of(max(p_lo, 0), max(p_hi, 0), p.window, p.sinks, kTileKeys);
     const int n = p_hi < 0 ? 0 : range.n;
     auto keys_of = [&](int j) {  // of tile j: up to the last row's position, in whole MMA steps
@@ -427,8 +461,7 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
     };
 
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *s_q = base, *s_k = base + 2 * L::kTile, *s_v = s_k + kStages * L::kTile;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint8_t *s_q = base, *s_k = base + S::kTiles * L::kQTile, *s_v = s_k + kStages * L::kKTile;
     if (tid == 0) {
         mbar_init(&bars.q_full, PAGED ? tiles * kTileRows : 1);
         for (int i = 0; i < kStages; i++) {
@@ -437,22 +470,24 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
             mbar_init(&bars.v_full[i], PAGED ? kConverters : 1);
             mbar_init(&bars.v_empty[i], 1);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&bars.s_full[i], 1);
-            mbar_init(&bars.p_full[i][0], kTileRows);
-            mbar_init(&bars.p_full[i][1], kTileRows);
+        for (int i = 0; i < S::kTiles; i++) {
+            for (int b = 0; b < kBuffers; b++) {
+                mbar_init(&bars.s_full[i][b], 1);
+                mbar_init(&bars.p_full[i][b], kTileRows);
+            }
+            mbar_init(&bars.o_done[i], 1);
             mbar_init(&bars.o_full[i], 1);
         }
         for (int i = 0; i < kScaleSlots; i++) {
-            mbar_init(&bars.scales_full[i], kTileKeys / 16);
+            mbar_init(&bars.scales_full[i], kScaleKeys / 16);
             mbar_init(&bars.scales_empty[i], 1);
         }
         bars.v_top = 0;
         bars.abort = 0;
         fence_barrier_init();
     }
-    if (warp == 8) {
-        tmem_alloc(&bars.tmem, 512);
+    if (warp == S::kIssuer) {
+        tmem_alloc(&bars.tmem, S::kTmem);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -462,9 +497,9 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
     int *status = p.status;
     volatile int *abort = &bars.abort;
 
-    if (warp >= 8 && warp < 12) give_registers<T::kIssueRegs>();
+    if (S::kTrade && warp >= 8 && warp < 12) give_registers<S::kIssueRegs>();
     if (PAGED && warp >= 12) {
-        give_registers<T::kConvertRegs>();
+        give_registers<S::kConvertRegs>();
         if (n > 0) {
             // ---- codes to operands ----
             const Cache &c = p.paged.c;
@@ -495,9 +530,9 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                 const bool value = u & 1;
                 if (!live) return false;
                 if (j >= kStages && !mbar_wait(value ? &bars.v_empty[st] : &bars.k_empty[st], (j / kStages + 1) & 1, abort, status)) return false;
-                uint8_t *dst = (value ? s_v : s_k) + st * L::kTile;
+                uint8_t *dst = (value ? s_v : s_k) + st * L::kKTile;
 #pragma unroll
-                for (int i = 0; i < kMine; i++) put_codes<DP, FP8>(dst, r0 + i * (kConverters / kChunks), chunk16, x[i]);
+                for (int i = 0; i < kMine; i++) put_codes<FP8>(dst, L::kKHalf, r0 + i * (kConverters / kChunks), chunk16, x[i]);
                 fence_proxy_async_smem();
                 mbar_arrive(value ? &bars.v_full[st] : &bars.k_full[st]);
                 return true;
@@ -510,7 +545,7 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                 if (!put(u + 1, buf[1])) break;
             }
         }
-    } else if (PAGED && warp == 9) {
+    } else if (PAGED && warp == S::kLoader) {
         if (n > 0) {
             // ---- pages and scales ----
             const Cache &c = p.paged.c;
@@ -552,104 +587,87 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                     mbar_arrive(&bars.scales_full[slot]);
                 }
         }
-    } else if (warp == 9) {
+    } else if (warp == S::kLoader) {
         if (lane == 0 && n > 0) {
             const int head0 = kvh * group + chunk * tl.heads;
             mbar_arrive_expect_tx(&bars.q_full, tiles * (DP / 64) * tl.heads * tl.toks * 128);
             for (int t = 0; t < tiles; t++)
 #pragma unroll
                 for (int h = 0; h < DP / 64; h++)
-                    tma_load_rows(&q_map, &bars.q_full, s_q + t * L::kTile + h * L::kHalf, 64 * h, head0, sq.q0 + i0 + t * tl.toks);
+                    tma_load_rows(&q_map, &bars.q_full, s_q + t * L::kQTile + h * L::kQHalf, 64 * h, head0, sq.q0 + i0 + t * tl.toks);
             for (int j = 0; j < n; j++) {
                 const int st = j % kStages, at = sq.k0 + range.token(j, kTileKeys);
-                const int boxes = (keys_of(j) + kBoxKeys - 1) / kBoxKeys;
                 for (int kv = 0; kv < 2; kv++) {
                     uint64_t *full = kv ? &bars.v_full[st] : &bars.k_full[st], *empty = kv ? &bars.v_empty[st] : &bars.k_empty[st];
                     if (j >= kStages && !mbar_wait(empty, (j / kStages + 1) & 1, abort, status)) goto loads_done;
-                    mbar_arrive_expect_tx(full, boxes * (DP / 64) * kBoxKeys * 128);
-                    uint8_t *dst = (kv ? s_v : s_k) + st * L::kTile;
-                    for (int b = 0; b < boxes; b++)
+                    mbar_arrive_expect_tx(full, L::kKTile);
+                    uint8_t *dst = (kv ? s_v : s_k) + st * L::kKTile;
 #pragma unroll
-                        for (int h = 0; h < DP / 64; h++)
-                            tma_load_rows(kv ? &v_map : &k_map, full, dst + h * L::kHalf + b * kBoxKeys * 128, 64 * h, kvh,
-                                          at + b * kBoxKeys);
+                    for (int h = 0; h < DP / 64; h++)
+                        tma_load_rows(kv ? &v_map : &k_map, full, dst + h * L::kKHalf, 64 * h, kvh, at);
                 }
             }
         loads_done:;
         }
-    } else if (warp == 8) {
+    } else if (warp == S::kIssuer) {
         if (n > 0) {
             constexpr uint32_t kType = BF16 && !PAGED ? 1 : 0;
             const bool leader = elect_one();
             const uint32_t q_at = smem_u32(s_q), k_at = smem_u32(s_k), v_at = smem_u32(s_v);
             auto qk = [&](int t, int j) {
                 const uint32_t id = idesc_of(kType, false, keys_of(j));
-                const uint64_t a = sw128_kmajor_desc(q_at + t * L::kTile), b = sw128_kmajor_desc(k_at + (j % kStages) * L::kTile);
-                const uint32_t d = tmem + 128 * t;
+                const uint64_t a = sw128_kmajor_desc(q_at + t * L::kQTile), b = sw128_kmajor_desc(k_at + (j % kStages) * L::kKTile);
+                const uint32_t d = tmem + 128 * t + kTileKeys * (j % kBuffers);
                 if (leader) {
 #pragma unroll
                     for (int h = 0; h < DP / 64; h++)
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            tc_mma_bf16(d, a + (h * L::kHalf >> 4) + 2 * k, b + (h * L::kHalf >> 4) + 2 * k, id, (h | k) ? 1u : 0u);
-                    tc_commit(&bars.s_full[t]);
+                            tc_mma_bf16(d, a + (h * L::kQHalf >> 4) + 2 * k, b + (h * L::kKHalf >> 4) + 2 * k, id, (h | k) ? 1u : 0u);
+                    tc_commit(&bars.s_full[t][j % kBuffers]);
+                    if (t == tiles - 1) tc_commit(&bars.k_empty[j % kStages]);
                 }
                 __syncwarp();
             };
-            auto commit = [&](uint64_t *bar) {
-                if (leader) tc_commit(bar);
-                __syncwarp();
-            };
-            bool ok = mbar_wait(&bars.q_full, 0, abort, status) && mbar_wait(&bars.k_full[0], 0, abort, status);
-            if (ok) {
+            bool ok = mbar_wait(&bars.q_full, 0, abort, status);
+            for (int j = 0; ok && j < min(kBuffers, n); j++) {
+                ok = mbar_wait(&bars.k_full[j], 0, abort, status);
+                if (!ok) break;
                 tc_fence_after();
-                for (int t = 0; t < tiles; t++) qk(t, 0);
-                commit(&bars.k_empty[0]);
+                for (int t = 0; t < tiles; t++) qk(t, j);
             }
             for (int j = 0; ok && j < n; j++) {
                 const int st = j % kStages, steps = keys_of(j) / 16;
                 for (int t = 0; ok && t < tiles; t++) {
-                    const uint32_t id = idesc_of(kType, true, DP), d = tmem + 256 + 128 * t, a = tmem + 128 * t;
-                    const uint64_t v = sw128_mnmajor_desc(v_at + st * L::kTile, L::kHalf);
-                    for (int half = 0; ok && half < 2; half++) {  // P comes in halves of 64 keys
-                        ok = mbar_wait(&bars.p_full[t][half], j & 1, abort, status);
-                        if (ok && t == 0 && half == 0) ok = mbar_wait(&bars.v_full[st], (j / kStages) & 1, abort, status);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (leader) {
-#pragma unroll
-                            for (int k = 0; k < 4; k++)
-                                if (4 * half + k < steps)
-                                    tc_mma_ts(d, a + 8 * (4 * half + k), v + (4 * half + k) * (16 * 128 >> 4), id, (j | half | k) ? 1u : 0u);
-                        }
-                        __syncwarp();
-                    }
+                    const uint32_t id = idesc_of(kType, true, DP), d = tmem + 128 * (S::kTiles + t), a = tmem + 128 * t + kTileKeys * (j % kBuffers);
+                    const uint64_t v = sw128_mnmajor_desc(v_at + st * L::kKTile, L::kKHalf);
+                    ok = mbar_wait(&bars.p_full[t][j % kBuffers], (j / kBuffers) & 1, abort, status);
+                    if (ok && t == 0) ok = mbar_wait(&bars.v_full[st], (j / kStages) & 1, abort, status);
+                    if (ok && t == 0 && j + kBuffers < n) ok = mbar_wait(&bars.k_full[(j + kBuffers) % kStages], ((j + kBuffers) / kStages) & 1, abort, status);
                     if (!ok) break;
-                    if (t == tiles - 1) {
-                        commit(&bars.v_empty[st]);
-                        if (PAGED) commit(&bars.scales_empty[j % kScaleSlots]);
-                    }
-                    if (j + 1 < n) {
-                        if (t == 0) {
-                            ok = mbar_wait(&bars.k_full[(j + 1) % kStages], ((j + 1) / kStages) & 1, abort, status);
-                            if (!ok) break;
-                            tc_fence_after();
+                    tc_fence_after();
+                    if (leader) {
+#pragma unroll
+                        for (int k = 0; k < kTileKeys / 16; k++)
+                            if (k < steps) tc_mma_ts(d, a + 8 * k, v + k * (16 * 128 >> 4), id, (j | k) ? 1u : 0u);
+                        tc_commit(j + 1 < n ? &bars.o_done[t] : &bars.o_full[t]);
+                        if (t == tiles - 1) {
+                            tc_commit(&bars.v_empty[st]);
+                            if (PAGED) tc_commit(&bars.scales_empty[j % kScaleSlots]);
                         }
-                        qk(t, j + 1);
-                        if (t == tiles - 1) commit(&bars.k_empty[(j + 1) % kStages]);
-                    } else {
-                        commit(&bars.o_full[t]);
                     }
+                    __syncwarp();
+                    if (j + kBuffers < n) qk(t, j + kBuffers);
                 }
             }
         }
-    } else if (warp < 8) {
-        take_registers<T::kSoftmaxRegs>();
+    } else if (warp < 4 * S::kTiles) {
+        if (S::kTrade) take_registers<S::kSoftmaxRegs>();
         if ((warp >> 2) < tiles) {
         // ---- softmax of tile t: this thread's row ----
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + 256 + 128 * t;
+        const uint32_t s_cols = tmem + lanes + 128 * t, o_at = tmem + lanes + 128 * (S::kTiles + t);
         const int tok = row / tl.heads, head = row - tok * tl.heads;  // of the tile
         const int i = i0 + t * tl.toks + tok, pos = first + i;
         const bool valid = tok < tl.toks && i < sq.nq && chunk * tl.heads + head < group;
@@ -671,7 +689,7 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
             e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
             const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
             c *= __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
-            uint8_t *dst = s_q + t * L::kTile + row * 128;
+            uint8_t *dst = s_q + t * L::kQTile + row * 128;
 #pragma unroll
             for (int d = 0; d < DP; d += 8) {
                 float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
@@ -679,7 +697,7 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                     x = load4(p.q, at + d);
                     y = load4(p.q, at + d + 4);
                 }
-                *reinterpret_cast<uint4 *>(dst + (d >> 6) * L::kHalf + ((((d & 63) >> 3) ^ (row & 7)) << 4)) =
+                *reinterpret_cast<uint4 *>(dst + (d >> 6) * L::kQHalf + ((((d & 63) >> 3) ^ (row & 7)) << 4)) =
                     make_uint4(pack16<false>(x.x * down, x.y * down), pack16<false>(x.z * down, x.w * down),
                                pack16<false>(y.x * down, y.y * down), pack16<false>(y.z * down, y.w * down));
             }
@@ -689,35 +707,36 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
         float m = -INFINITY, l = 0.0f;  // m: the reference maximum of score * c, in base 2
         bool ok = true;
         for (int j = 0; j < n; j++) {
-            if (!mbar_wait(&bars.s_full[t], j & 1, abort, status)) {
+            const uint32_t s_at = s_cols + kTileKeys * (j % kBuffers);
+            if (!mbar_wait(&bars.s_full[t][j % kBuffers], (j / kBuffers) & 1, abort, status)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            uint32_t s[128];
+            uint32_t s[kTileKeys];
 #pragma unroll
-            for (int b = 0; b < 4; b++) tmem_ld32_start(s_at + 32 * b, s + 32 * b);
+            for (int b = 0; b < kTileKeys; b += 32) tmem_ld32_start(s_at + b, s + b);
             tmem_ld_wait();
             const int k0 = range.token(j, kTileKeys);
             if (k0 + kTileKeys - 1 > t_lo || (p.window && k0 <= t_hi - p.window)) {
                 const int hi = pos - k0, lo = p.window ? hi - p.window + 1 : 0, sink = p.sinks - k0;
 #pragma unroll
-                for (int b = 0; b < 128; b++)
+                for (int b = 0; b < kTileKeys; b++)
                     if (b > hi || (b < lo && b >= sink)) s[b] = 0xff800000u;
             }
-            float f[8];  // factor of the scores of 16 keys
+            float f[kTileKeys / 16];  // factor of the scores of 16 keys
             if (PAGED) {
                 if (!mbar_wait(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, abort, status)) {
                     ok = false;
                     break;
                 }
 #pragma unroll
-                for (int b = 0; b < 8; b++) f[b] = c * bars.sk[j % kScaleSlots][b];
+                for (int b = 0; b < kTileKeys / 16; b++) f[b] = c * bars.sk[j % kScaleSlots][b];
             }
             float mx = -INFINITY;
             if (PAGED) {
 #pragma unroll
-                for (int b = 0; b < 8; b++) {
+                for (int b = 0; b < kTileKeys / 16; b++) {
                     float x = __uint_as_float(s[16 * b]), y = __uint_as_float(s[16 * b + 1]);
 #pragma unroll
                     for (int e = 2; e < 14; e += 4) {
@@ -730,7 +749,7 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
             } else {
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int b = 0; b < 128; b += 8)
+                for (int b = 0; b < kTileKeys; b += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++) top[e] = max3(top[e], __uint_as_float(s[b + e]), __uint_as_float(s[b + 4 + e]));
                 mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
@@ -740,7 +759,12 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                 const float keep = m == -INFINITY ? 0.0f : exp2f(m - to);
                 m = to;
                 l *= keep;
-                if (j > 0) {
+                if (j > 0) {  // (P.V(j) is not before this row's P, so this is the phase under way or the last)
+                    if (!mbar_wait(&bars.o_done[t], (j - 1) & 1, abort, status)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
 #pragma unroll
                     for (int b = 0; b < DP; b += 32) {
                         uint32_t o[32];
@@ -754,10 +778,9 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
             }
             const float ref = m == -INFINITY ? 0.0f : -m;
             f32x2 sum[2] = {0, 0};
-            // by quarters of 32 keys; the first half of P is handed over while the last quarter is made
-            uint32_t w[32];
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
+            for (int b = 0; b < kTileKeys / 32; b++) {
+                uint32_t w[16];
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
                     const int at = 32 * b + 16 * q;
@@ -776,25 +799,20 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
                         }
                         f32x2 &to = PAGED ? part[e & 1] : sum[e & 1];
                         to = add2(to, pair_of(a.x, a.y));
-                        w[16 * (b & 1) + 8 * q + e] = pack16<BF16 && !PAGED>(a.x, a.y);
+                        w[8 * q + e] = pack16<BF16 && !PAGED>(a.x, a.y);
                     }
                     if (PAGED) {
                         const float iv = bars.iv[j % kScaleSlots][2 * b + q];
                         sum[q] = fma2(add2(part[0], part[1]), pair_of(iv, iv), sum[q]);
                     }
                 }
-                if (b == 2) {
-                    tmem_st_wait();
-                    tc_fence_before();
-                    mbar_arrive(&bars.p_full[t][0]);
-                }
-                if (b & 1) tmem_st32(s_at + 16 * (b - 1), w);
+                tmem_st16_start(s_at + 16 * b, w);
             }
             const float2 s2 = floats_of(add2(sum[0], sum[1]));
             l += s2.x + s2.y;
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&bars.p_full[t][1]);
+            mbar_arrive(&bars.p_full[t][j % kBuffers]);
         }
         // ---- out = O / l ----
         if (ok && n > 0) {
@@ -841,9 +859,9 @@ __global__ void __launch_bounds__(Team<PAGED>::kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == S::kIssuer) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, S::kTmem);
     }
 }
 
@@ -863,21 +881,30 @@ Tiling tiling_of(int group) {
     return tl;
 }
 
-template <int DP, bool BF16, bool PAGED, bool FP8>
+template <int DP, bool BF16, bool FP8, class S>
 cudaError_t launch(const TiledParams &p, cudaStream_t s) {
     const Tiling tl = tiling_of(p.q.heads / p.kv_heads);
     CUtensorMap q{}, k{}, v{};
-    if (!PAGED && (!rows_map(&q, p.q, p.dim, p.n_q, tl.heads, tl.toks) || !rows_map(&k, p.rows.k, p.dim, p.rows.n_kv, 1, kBoxKeys) ||
-                   !rows_map(&v, p.rows.v, p.dim, p.rows.n_kv, 1, kBoxKeys)))
+    if (!S::kPaged && (!rows_map(&q, p.q, p.dim, p.n_q, tl.heads, tl.toks) ||
+                       !rows_map(&k, p.rows.k, p.dim, p.rows.n_kv, 1, S::kKeys) || !rows_map(&v, p.rows.v, p.dim, p.rows.n_kv, 1, S::kKeys)))
         return cudaErrorInvalidValue;
     static SmemOptIn opt_in;
-    const cudaError_t e = opt_in.set(reinterpret_cast<const void *>(k_tiled<DP, BF16, PAGED, FP8>), WinLayout<DP>::kBytes);
+    const cudaError_t e = opt_in.set(reinterpret_cast<const void *>(k_tiled<DP, BF16, FP8, S>), Layout<DP, S>::kBytes);
     if (e != cudaSuccess) return e;
-    const int pairs = (p.max_q + 2 * tl.toks - 1) / (2 * tl.toks);
-    const long long nx = (long long)p.n_seqs * p.kv_heads * tl.chunks;
-    if (pairs > 65535 || nx > 0x7fffffffLL) return cudaErrorInvalidValue;
-    k_tiled<DP, BF16, PAGED, FP8><<<dim3((unsigned)nx, (unsigned)pairs), Team<PAGED>::kThreads, WinLayout<DP>::kBytes, s>>>(q, k, v, p, tl, pairs);
+    const int pairs = (p.max_q + S::kTiles * tl.toks - 1) / (S::kTiles * tl.toks);
+    const long long nx = (long long)pairs * p.kv_heads * tl.chunks;
+    if (p.n_seqs > 65535 || nx > 0x7fffffffLL) return cudaErrorInvalidValue;
+    k_tiled<DP, BF16, FP8, S><<<dim3((unsigned)nx, (unsigned)p.n_seqs), S::kThreads, Layout<DP, S>::kBytes, s>>>(q, k, v, p, tl, pairs);
     return cudaGetLastError();
+}
+
+// Keys in sight of a row from which the shape with the least MMA time wins.
+constexpr long long kLongRun = 2048;
+
+template <int DP, bool BF16>
+cudaError_t launch_rows(const TiledParams &p, long long seen, cudaStream_t s) {
+    if (seen >= kLongRun) return launch<DP, BF16, false, Shape<false, 128, 2>>(p, s);
+    return launch<DP, BF16, false, Shape<false, 64, 1>>(p, s);
 }
 
 }  // namespace
@@ -902,15 +929,19 @@ cudaError_t window_attention(const WindowParams &w, int, cudaStream_t s) {
         k_window_rows<<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
         return cudaGetLastError();
     }
-    if (p.q.dtype == kBf16) return p.dim <= 64 ? launch<64, true, false, false>(p, s) : launch<128, true, false, false>(p, s);
-    return p.dim <= 64 ? launch<64, false, false, false>(p, s) : launch<128, false, false, false>(p, s);
+    long long seen = w.b.max_kv;
+    if (p.window) seen = std::min<long long>(seen, (long long)p.window + p.sinks);
+    if (p.q.dtype == kBf16) return p.dim <= 64 ? launch_rows<64, true>(p, seen, s) : launch_rows<128, true>(p, seen, s);
+    return p.dim <= 64 ? launch_rows<64, false>(p, seen, s) : launch_rows<128, false>(p, seen, s);
 }
+
+using CacheShape = Shape<true, 64, 2>;
 
 // Rounds of CTAs, one to an SM, times tiles of keys.
 double tiled_rounds(const AttendParams &a, int sms, long long seen) {
     const Tiling tl = tiling_of(a.q.heads / a.c.heads);
     const long long items = (long long)a.b.n_seqs * a.c.heads * tl.chunks * ((a.b.max_new + 2 * tl.toks - 1) / (2 * tl.toks));
-    return (double)((items + sms - 1) / sms) * ((seen + kTileKeys - 1) / kTileKeys);
+    return (double)((items + sms - 1) / sms) * ((seen + CacheShape::kKeys - 1) / CacheShape::kKeys);
 }
 
 cudaError_t attend_tiled(const AttendParams &a, cudaStream_t s) {
@@ -929,11 +960,11 @@ cudaError_t attend_tiled(const AttendParams &a, cudaStream_t s) {
     p.paged = Paged{a.c, a.b};
     const bool bf16 = a.out.dtype == kBf16;
     if (p.dim <= 64) {
-        if (a.c.fp8) return bf16 ? launch<64, true, true, true>(p, s) : launch<64, false, true, true>(p, s);
-        return bf16 ? launch<64, true, true, false>(p, s) : launch<64, false, true, false>(p, s);
+        if (a.c.fp8) return bf16 ? launch<64, true, true, CacheShape>(p, s) : launch<64, false, true, CacheShape>(p, s);
+        return bf16 ? launch<64, true, false, CacheShape>(p, s) : launch<64, false, false, CacheShape>(p, s);
     }
-    if (a.c.fp8) return bf16 ? launch<128, true, true, true>(p, s) : launch<128, false, true, true>(p, s);
-    return bf16 ? launch<128, true, true, false>(p, s) : launch<128, false, true, false>(p, s);
+    if (a.c.fp8) return bf16 ? launch<128, true, true, CacheShape>(p, s) : launch<128, false, true, CacheShape>(p, s);
+    return bf16 ? launch<128, true, false, CacheShape>(p, s) : launch<128, false, false, CacheShape>(p, s);
 }
 
 }  // namespace kv

@@ -414,6 +414,10 @@ WINDOWS = [
     ("bf16", 130, 1, 64, [(9, 50)], 0, 0),
     ("f16", 4, 4, 8, [(300, 300)], 200, 150),
     ("bf16", 28, 4, 128, [(1, 2000), (2, 1999)], 0, 0),
+    # runs of 2048 keys and more: the shape for long runs, with ragged ends (one row tile, few keys)
+    ("bf16", 8, 2, 128, [(300, 2500), (33, 70), (1, 1), (40, 2049)], 0, 0),
+    ("f16", 14, 2, 64, [(95, 3001), (18, 18), (19, 500)], 2500, 4),
+    ("bf16", 4, 4, 80, [(129, 129), (2100, 2100)], 0, 0),
 ]
 
 
