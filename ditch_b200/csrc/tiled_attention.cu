@@ -215,7 +215,8 @@ constexpr int kMostStages = 4, kScaleKeys = 64;  // (the cache's tiles are of 64
 
 struct Bars {
     uint64_t q_full, k_full[kMostStages], k_empty[kMostStages], v_full[kMostStages], v_empty[kMostStages];
-    uint64_t s_full[2][2], p_full[2][2], o_done[2], o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
+    uint64_t s_full[2][2], p_full[2][2],  // P of the two tiles of 64 keys, or of the two halves of 128
+         o_done[2], o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
     // per 16 keys of a tile: the factor of scores, log2 of sv / the largest sv, its inverse
     // and the offset of their codes (-1: none)
     long long codes[kScaleSlots][kScaleKeys / 16];
@@ -357,33 +358,6 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
     return r;
 }
 
-// 2^x of two numbers not above 2^7 on the FMA pipe, for a share of the
-// exponentials, of which the SFU makes only 16 a cycle: x = n + r with n an
-// integer (rounding by adding 1.5 * 2^23), 2^r on [-1/2, 1/2] by the
-// polynomial of degree 4 with the smallest largest relative error (2.6e-6, by
-// iteratively reweighted least squares), n added to the exponent. Numbers
-// below -126 give 2^-126; a NaN gives something that is not finite in 16 bits.
-__device__ __forceinline__ float2 exp2_fma(f32x2 x) {
-    const float2 v = floats_of(x);
-    float lo, hi;
-    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(lo) : "f"(v.x));
-    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(hi) : "f"(v.y));
-    x = pair_of(lo, hi);
-    const f32x2 n = add2(x, pair_of(12582912.0f, 12582912.0f));
-    const f32x2 r = fma2(add2(n, pair_of(-12582912.0f, -12582912.0f)), pair_of(-1.0f, -1.0f), x);
-    f32x2 y = pair_of(0.009570102207362652f, 0.009570102207362652f);
-    y = fma2(y, r, pair_of(0.05591786280274391f, 0.05591786280274391f));
-    y = fma2(y, r, pair_of(0.240247443318367f, 0.240247443318367f));
-    y = fma2(y, r, pair_of(0.6931217908859253f, 0.6931217908859253f));
-    y = fma2(y, r, pair_of(0.9999992847442627f, 0.9999992847442627f));
-    const float2 p = floats_of(y), k = floats_of(n);
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(k.x) << 23)),
-                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(k.y) << 23)));
-}
-
-// Which of the eight pairs of 16 keys take the FMA pipe.
-constexpr uint32_t kByFma = 0x00;
-
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     if (BF16) return pack_bf16x2(lo, hi);
@@ -473,8 +447,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         for (int i = 0; i < S::kTiles; i++) {
             for (int b = 0; b < kBuffers; b++) {
                 mbar_init(&bars.s_full[i][b], 1);
-                mbar_init(&bars.p_full[i][b], kTileRows);
             }
+            for (int b = 0; b < 2; b++) mbar_init(&bars.p_full[i][b], kTileRows);
             mbar_init(&bars.o_done[i], 1);
             mbar_init(&bars.o_full[i], 1);
         }
@@ -641,15 +615,23 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 for (int t = 0; ok && t < tiles; t++) {
                     const uint32_t id = idesc_of(kType, true, DP), d = tmem + 128 * (S::kTiles + t), a = tmem + 128 * t + kTileKeys * (j % kBuffers);
                     const uint64_t v = sw128_mnmajor_desc(v_at + st * L::kKTile, L::kKHalf);
-                    ok = mbar_wait(&bars.p_full[t][j % kBuffers], (j / kBuffers) & 1, abort, status);
-                    if (ok && t == 0) ok = mbar_wait(&bars.v_full[st], (j / kStages) & 1, abort, status);
+                    if (t == 0) ok = mbar_wait(&bars.v_full[st], (j / kStages) & 1, abort, status);
                     if (ok && t == 0 && j + kBuffers < n) ok = mbar_wait(&bars.k_full[(j + kBuffers) % kStages], ((j + kBuffers) / kStages) & 1, abort, status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (leader) {
 #pragma unroll
-                        for (int k = 0; k < kTileKeys / 16; k++)
-                            if (k < steps) tc_mma_ts(d, a + 8 * k, v + k * (16 * 128 >> 4), id, (j | k) ? 1u : 0u);
+                    for (int half = 0; half < kTileKeys / 64; half++) {
+                        if (!ok) break;
+                        ok = mbar_wait(&bars.p_full[t][kBuffers == 2 ? j & 1 : half], (j / kBuffers) & 1, abort, status);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (leader) {
+#pragma unroll
+                            for (int k = 4 * half; k < 4 * half + 4; k++)
+                                if (k < steps) tc_mma_ts(d, a + 8 * k, v + k * (16 * 128 >> 4), id, (j | k) ? 1u : 0u);
+                        }
+                        __syncwarp();
+                    }
+                    if (!ok) break;
+                    if (leader) {
                         tc_commit(j + 1 < n ? &bars.o_done[t] : &bars.o_full[t]);
                         if (t == tiles - 1) {
                             tc_commit(&bars.v_empty[st]);
@@ -790,13 +772,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const f32x2 x = fma2(pair_of(__uint_as_float(s[at + 2 * e]), __uint_as_float(s[at + 2 * e + 1])), f2, r2);
-                        float2 a;
-                        if (kByFma >> e & 1) {
-                            a = exp2_fma(x);
-                        } else {
-                            const float2 v = floats_of(x);
-                            a = make_float2(exp2_sfu(v.x), exp2_sfu(v.y));
-                        }
+                        const float2 v = floats_of(x), a = make_float2(exp2_sfu(v.x), exp2_sfu(v.y));
                         f32x2 &to = PAGED ? part[e & 1] : sum[e & 1];
                         to = add2(to, pair_of(a.x, a.y));
                         w[8 * q + e] = pack16<BF16 && !PAGED>(a.x, a.y);
@@ -806,13 +782,18 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         sum[q] = fma2(add2(part[0], part[1]), pair_of(iv, iv), sum[q]);
                     }
                 }
+                if (kTileKeys == 128 && b == 2) {  // P.V of the first half may begin
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&bars.p_full[t][0]);
+                }
                 tmem_st16_start(s_at + 16 * b, w);
             }
             const float2 s2 = floats_of(add2(sum[0], sum[1]));
             l += s2.x + s2.y;
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&bars.p_full[t][j % kBuffers]);
+            mbar_arrive(&bars.p_full[t][kBuffers == 2 ? j & 1 : 1]);
         }
         // ---- out = O / l ----
         if (ok && n > 0) {
@@ -820,7 +801,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             tc_fence_after();
         }
         if (ok) {
-            float inv = m == -INFINITY && l == l ? 0.0f : 1.0f / l;  // (hidden weights may be 2^-126)
+            float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
             if (PAGED && n > 0) inv *= __uint_as_float(bars.v_top);
             const long long at = (sq.q0 + i) * p.out.ts + (kvh * group + chunk * tl.heads + head) * p.out.hs;
             bool odd = false;  // something is not finite
