@@ -185,6 +185,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_window_rows(TiledParams p) {
 // ---- the tiled kernel ------------------------------------------------------------------
 constexpr int kTileRows = 128;  // query rows of a tile: the MMA's M, a TMEM lane each
 
+constexpr int kConverters = 128;  // threads that turn codes into operands
+
 // KEYS: of a tile; TILES: row tiles of a CTA.
 template <bool PAGED_, int KEYS_, int TILES_>
 struct Shape {
@@ -195,13 +197,12 @@ struct Shape {
     // Registers that the softmax warps take from the others at the start (setmaxnreg; 512 threads begin with 128
     // each, 384 with 168): they hold a row of scores. With 64 keys and no converters, what they begin with is enough.
     static constexpr bool kTrade = PAGED_ || KEYS_ == 128;
-    static constexpr int kThreads = PAGED_ ? 512 : kTrade ? 384 : 128 * TILES_ + 64;
+    static constexpr int kThreads = PAGED_ ? 384 + kConverters : kTrade ? 384 : 128 * TILES_ + 64;
     static constexpr int kSoftmaxRegs = PAGED_ ? 160 : 208, kIssueRegs = 80, kConvertRegs = 112;
     static constexpr int kCtas = TILES_ == 1 ? 2 : 1;                  // an SM
     static constexpr int kIssuer = 4 * TILES_, kLoader = kIssuer + 1;  // warps
     static constexpr uint32_t kTmem = 256 * TILES_;
 };
-constexpr int kConverters = 128;  // threads that turn codes into operands
 constexpr int kScaleSlots = 8;    // tiles whose pages and scales are known at a time
 
 template <int DP, class S>
@@ -216,7 +217,7 @@ constexpr int kMostStages = 4, kScaleKeys = 64;  // (the cache's tiles are of 64
 struct Bars {
     uint64_t q_full, k_full[kMostStages], k_empty[kMostStages], v_full[kMostStages], v_empty[kMostStages];
     uint64_t s_full[2][2], p_full[2][2],  // P of the two tiles of 64 keys, or of the two halves of 128
-         o_done[2], o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
+         o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
     // per 16 keys of a tile: the factor of scores, log2 of sv / the largest sv, its inverse
     // and the offset of their codes (-1: none)
     long long codes[kScaleSlots][kScaleKeys / 16];
@@ -436,7 +437,33 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *s_q = base, *s_k = base + S::kTiles * L::kQTile, *s_v = s_k + kStages * L::kKTile;
-    if (tid == 0) {
+    // Contiguous rows: Q, and K (kv 0) or V (kv 1) of tile j.
+    auto load = [&](int kv, int j) {
+        uint64_t *full = kv ? &bars.v_full[j % kStages] : &bars.k_full[j % kStages];
+        mbar_arrive_expect_tx(full, L::kKTile);
+        uint8_t *dst = (kv ? s_v : s_k) + j % kStages * L::kKTile;
+#pragma unroll
+        for (int h = 0; h < DP / 64; h++)
+            tma_load_rows(kv ? &v_map : &k_map, full, dst + h * L::kKHalf, 64 * h, kvh, sq.k0 + range.token(j, kTileKeys));
+    };
+    auto load_first = [&]() {
+        const int head0 = kvh * group + chunk * tl.heads;
+        mbar_arrive_expect_tx(&bars.q_full, tiles * (DP / 64) * tl.heads * tl.toks * 128);
+        for (int t = 0; t < tiles; t++)
+#pragma unroll
+            for (int h = 0; h < DP / 64; h++)
+                tma_load_rows(&q_map, &bars.q_full, s_q + t * L::kQTile + h * L::kQHalf, 64 * h, head0, sq.q0 + i0 + t * tl.toks);
+        for (int j = 0; j < min(n, kStages); j++) {
+            load(0, j);
+            load(1, j);
+        }
+    };
+    if (warp == S::kLoader && lane == 0) {
+        if (!PAGED) {
+            tma_prefetch_desc(&q_map);
+            tma_prefetch_desc(&k_map);
+            tma_prefetch_desc(&v_map);
+        }
         mbar_init(&bars.q_full, PAGED ? tiles * kTileRows : 1);
         for (int i = 0; i < kStages; i++) {
             mbar_init(&bars.k_full[i], PAGED ? kConverters : 1);
@@ -449,7 +476,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 mbar_init(&bars.s_full[i][b], 1);
             }
             for (int b = 0; b < 2; b++) mbar_init(&bars.p_full[i][b], kTileRows);
-            mbar_init(&bars.o_done[i], 1);
             mbar_init(&bars.o_full[i], 1);
         }
         for (int i = 0; i < kScaleSlots; i++) {
@@ -459,6 +485,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         bars.v_top = 0;
         bars.abort = 0;
         fence_barrier_init();
+        if (!PAGED && n > 0) load_first();
     }
     if (warp == S::kIssuer) {
         tmem_alloc(&bars.tmem, S::kTmem);
@@ -535,9 +562,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             top = __reduce_max_sync(0xffffffffu, top);
             if (lane == 0) bars.v_top = top;
             const float v_top = __uint_as_float(top);
-            if (lane < kTileKeys / 16)
-                for (int j = 0; j < n; j++) {
-                    const int key = range.token(j, kTileKeys) + 16 * lane, slot = j % kScaleSlots;
+            // a lane for each 16 keys of eight tiles, so that the loads' latencies are paid once for all of them
+            static_assert(kScaleSlots * (kScaleKeys / 16) == 32, "a lane each");
+            const int block = lane % (kScaleKeys / 16);
+            for (int j = lane / (kScaleKeys / 16); j < n; j += kScaleSlots) {
+                    const int key = range.token(j, kTileKeys) + 16 * block, slot = j % kScaleSlots;
                     float sk = 0.0f, sv = 0.0f;
                     long long codes = -1;
                     if (key <= p_hi) {
@@ -554,34 +583,21 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                     float ratio = sv / v_top;
                     if (!(ratio >= 0x1p-40f)) ratio = ratio != ratio && v_top != 0.0f ? ratio : 0x1p-40f;
                     if (j >= kScaleSlots && !mbar_wait(&bars.scales_empty[slot], (j / kScaleSlots + 1) & 1, abort, status)) break;
-                    bars.codes[slot][lane] = codes;
-                    bars.sk[slot][lane] = sk == 0.0f ? 0x1p-100f : sk;
-                    bars.lv[slot][lane] = log2f(ratio);
-                    bars.iv[slot][lane] = 1.0f / ratio;
+                    bars.codes[slot][block] = codes;
+                    bars.sk[slot][block] = sk == 0.0f ? 0x1p-100f : sk;
+                    bars.lv[slot][block] = log2f(ratio);
+                    bars.iv[slot][block] = 1.0f / ratio;
                     mbar_arrive(&bars.scales_full[slot]);
                 }
         }
     } else if (warp == S::kLoader) {
         if (lane == 0 && n > 0) {
-            const int head0 = kvh * group + chunk * tl.heads;
-            mbar_arrive_expect_tx(&bars.q_full, tiles * (DP / 64) * tl.heads * tl.toks * 128);
-            for (int t = 0; t < tiles; t++)
-#pragma unroll
-                for (int h = 0; h < DP / 64; h++)
-                    tma_load_rows(&q_map, &bars.q_full, s_q + t * L::kQTile + h * L::kQHalf, 64 * h, head0, sq.q0 + i0 + t * tl.toks);
-            for (int j = 0; j < n; j++) {
-                const int st = j % kStages, at = sq.k0 + range.token(j, kTileKeys);
-                for (int kv = 0; kv < 2; kv++) {
-                    uint64_t *full = kv ? &bars.v_full[st] : &bars.k_full[st], *empty = kv ? &bars.v_empty[st] : &bars.k_empty[st];
-                    if (j >= kStages && !mbar_wait(empty, (j / kStages + 1) & 1, abort, status)) goto loads_done;
-                    mbar_arrive_expect_tx(full, L::kKTile);
-                    uint8_t *dst = (kv ? s_v : s_k) + st * L::kKTile;
-#pragma unroll
-                    for (int h = 0; h < DP / 64; h++)
-                        tma_load_rows(kv ? &v_map : &k_map, full, dst + h * L::kKHalf, 64 * h, kvh, at);
+            bool go = true;
+            for (int j = kStages; go && j < n; j++)
+                for (int kv = 0; go && kv < 2; kv++) {
+                    go = mbar_wait(kv ? &bars.v_empty[j % kStages] : &bars.k_empty[j % kStages], (j / kStages + 1) & 1, abort, status);
+                    if (go) load(kv, j);
                 }
-            }
-        loads_done:;
         }
     } else if (warp == S::kIssuer) {
         if (n > 0) {
@@ -610,13 +626,18 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 tc_fence_after();
                 for (int t = 0; t < tiles; t++) qk(t, j);
             }
+            // what the products of step j read besides P: V(j) and K(j + kBuffers)
+            auto operands = [&](int j) {
+                return mbar_wait(&bars.v_full[j % kStages], (j / kStages) & 1, abort, status) &&
+                       (j + kBuffers >= n ||
+                        mbar_wait(&bars.k_full[(j + kBuffers) % kStages], ((j + kBuffers) / kStages) & 1, abort, status));
+            };
+            ok = ok && operands(0);
             for (int j = 0; ok && j < n; j++) {
                 const int st = j % kStages, steps = keys_of(j) / 16;
                 for (int t = 0; ok && t < tiles; t++) {
                     const uint32_t id = idesc_of(kType, true, DP), d = tmem + 128 * (S::kTiles + t), a = tmem + 128 * t + kTileKeys * (j % kBuffers);
                     const uint64_t v = sw128_mnmajor_desc(v_at + st * L::kKTile, L::kKHalf);
-                    if (t == 0) ok = mbar_wait(&bars.v_full[st], (j / kStages) & 1, abort, status);
-                    if (ok && t == 0 && j + kBuffers < n) ok = mbar_wait(&bars.k_full[(j + kBuffers) % kStages], ((j + kBuffers) / kStages) & 1, abort, status);
 #pragma unroll
                     for (int half = 0; half < kTileKeys / 64; half++) {
                         if (!ok) break;
@@ -632,15 +653,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                     }
                     if (!ok) break;
                     if (leader) {
-                        tc_commit(j + 1 < n ? &bars.o_done[t] : &bars.o_full[t]);
-                        if (t == tiles - 1) {
-                            tc_commit(&bars.v_empty[st]);
-                            if (PAGED) tc_commit(&bars.scales_empty[j % kScaleSlots]);
-                        }
+                        if (t == tiles - 1) tc_commit(&bars.v_empty[st]);
+                        if (PAGED && t == tiles - 1) tc_commit(&bars.scales_empty[j % kScaleSlots]);
+                        if (j + 1 == n) tc_commit(&bars.o_full[t]);
                     }
                     __syncwarp();
                     if (j + kBuffers < n) qk(t, j + kBuffers);
                 }
+                if (ok && j + 1 < n) ok = operands(j + 1);  // while the MMAs are under way
             }
         }
     } else if (warp < 4 * S::kTiles) {
@@ -741,8 +761,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 const float keep = m == -INFINITY ? 0.0f : exp2f(m - to);
                 m = to;
                 l *= keep;
-                if (j > 0) {  // (P.V(j) is not before this row's P, so this is the phase under way or the last)
-                    if (!mbar_wait(&bars.o_done[t], (j - 1) & 1, abort, status)) {
+                if (j > 0) {  // P.V(j - 1) of all tiles is in (P.V(j) waits for this row, so no later phase can be over)
+                    if (!mbar_wait(&bars.v_empty[(j - 1) % kStages], ((j - 1) / kStages) & 1, abort, status)) {
                         ok = false;
                         break;
                     }
