@@ -54,6 +54,16 @@ __global__ void __launch_bounds__(kStoreWarps * 32) k_kv_store(KvParams p) {
     }
 }
 
+// A warp per (row, q or k head); a lane reads and writes only its own elements.
+__global__ void __launch_bounds__(kStoreWarps * 32) k_head_norms(float *qkv, int n, int heads, int kv_heads, int hd,
+                                                                 const float *q_norm, const float *k_norm, float eps) {
+    const long long x = (long long)blockIdx.x * kStoreWarps + (threadIdx.x >> 5);
+    const int per = heads + kv_heads, r = (int)(x / per), s = (int)(x - (long long)r * per);
+    if (r >= n) return;
+    rms_inplace(qkv + (long long)r * (heads + 2 * kv_heads) * hd + s * hd, hd, s < heads ? q_norm : k_norm, eps,
+                threadIdx.x & 31);
+}
+
 // ---- single-token attention over the cache --------------------------------
 // Block = (row, kv head). Keys and values 0..pos of the row's slot are staged
 // in shared memory kDecChunk at a time and shared by the group's q heads;
@@ -354,6 +364,14 @@ __global__ void __launch_bounds__(1024) k_argmax_rows(const float *x, int len, u
 }
 
 }  // namespace
+
+cudaError_t head_norms(float *qkv, int n, int heads, int kv_heads, int head_dim, const float *q_norm, const float *k_norm,
+                       float eps, cudaStream_t st) {
+    const long long warps = (long long)n * (heads + kv_heads);
+    k_head_norms<<<(unsigned)((warps + kStoreWarps - 1) / kStoreWarps), kStoreWarps * 32, 0, st>>>(qkv, n, heads, kv_heads,
+                                                                                                   head_dim, q_norm, k_norm, eps);
+    return cudaGetLastError();
+}
 
 cudaError_t kv_store(const KvParams &p, cudaStream_t st) {
     if (p.n <= 0) return cudaSuccess;

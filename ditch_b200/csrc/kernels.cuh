@@ -133,6 +133,9 @@ struct KvParams {
     int *status;
 };
 // Stores every row's keys and values at (slot, position) of the cache.
+// Per-head RMSNorm of the q and k heads of qkv rows, in place (qwen3-style).
+cudaError_t head_norms(float *qkv, int n, int heads, int kv_heads, int head_dim, const float *q_norm, const float *k_norm,
+                       float eps, cudaStream_t st);
 cudaError_t kv_store(const KvParams &p, cudaStream_t st);
 
 struct DecodeAttnParams {

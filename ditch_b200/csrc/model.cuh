@@ -145,6 +145,10 @@ struct ditch_cuda_model {
     // greedy generation: KV cache f32 [layers][slots][kv_len][kvd] for keys and for values
     ditch::DevBuf kv_k, kv_v, gen_next;
     int kv_slots = 0, kv_len = 0;
+    // the paged 8-bit cache (kv8_format -1: the f32 one): codes and scales of all layers, the sequences' arrays
+    int kv8_format = -1, kv8_pages = 0, kv8_seqs = 0, kv8_max_new = 0, kv8_max_len = 0;
+    size_t kv8_window = 0, kv8_sinks = 0, kv8_ws_zeroed = 0;
+    ditch::DevBuf kv8_k, kv8_v, kv8_ks, kv8_vs, kv8_off, kv8_len, kv8_table, kv8_ws, kv8_q16, kv8_k16, kv8_v16;
     int row_norm = 0;    // edit row normalisation: 0 none, 1 pre, 2 full (src/abliterate.zig:283-350)
     int lora_rank = 3;   // full: rank of the delta (Options.lora_rank)
     uint64_t edit_seed = 0, seed_counter = 0;  // full: the sketch seed of each matrix is seed + its index

@@ -6,6 +6,7 @@
 #include <array>
 #include <numeric>
 
+#include "kvcache.cuh"
 #include "model.cuh"
 
 using namespace ditch;
@@ -469,6 +470,113 @@ int gemm_mat(ditch_cuda_device *dev, const Mat &w, int slab_row0, int m_rows, co
     return DITCH_CUDA_OK;
 }
 
+constexpr int kKv8Page = 64, kKv8Block = 16;  // tokens of a page and of a scale
+
+// Layer li's pool and the current sequences of the paged 8-bit cache.
+static kv::Cache kv8_cache(ditch_cuda_model *m, int li) {
+    const Config &c = m->cfg;
+    const size_t pages = (size_t)m->kv8_pages, codes = pages * c.kvd() * kKv8Page, scales = pages * c.kv_heads * (kKv8Page / kKv8Block);
+    kv::Cache k{};
+    k.k = m->kv8_k.as<uint8_t>() + li * codes;
+    k.v = m->kv8_v.as<uint8_t>() + li * codes;
+    k.ks = m->kv8_ks.as<float>() + li * scales;
+    k.vs = m->kv8_vs.as<float>() + li * scales;
+    k.n_pages = m->kv8_pages;
+    k.fp8 = m->kv8_format == DITCH_KV_FP8;
+    k.heads = c.kv_heads;
+    k.dim = c.head_dim;
+    k.page_shift = 6;
+    k.block_shift = 4;
+    return k;
+}
+
+// The sequences of a step: rows[i] rows (the last of lens[i] tokens) for slot slots[i] of the cache.
+static int kv8_begin(ditch_cuda_model *m, const std::vector<int> &rows, const std::vector<int> &lens, const std::vector<int> &slots) {
+    cudaStream_t st = m->dev->stream;
+    const int per = (m->kv_len + kKv8Page - 1) / kKv8Page, n = (int)rows.size();
+    std::vector<int> off(n + 1, 0), table((size_t)n * per);
+    for (int i = 0; i < n; i++) {
+        off[i + 1] = off[i] + rows[i];
+        for (int k = 0; k < per; k++) table[(size_t)i * per + k] = slots[i] * per + k;
+    }
+    DITCH_CUDA(upload_vec(m->kv8_off, off, st));
+    DITCH_CUDA(upload_vec(m->kv8_len, lens, st));
+    DITCH_CUDA(upload_vec(m->kv8_table, table, st));
+    m->kv8_seqs = n;
+    m->kv8_max_new = *std::max_element(rows.begin(), rows.end());
+    m->kv8_max_len = *std::max_element(lens.begin(), lens.end());
+    return DITCH_CUDA_OK;
+}
+
+// Attention of one layer with the paged 8-bit cache: the QKV rows' keys and
+// values are appended (rotated on the way); a prefill attends over its own
+// rows in bf16, a decode step over the cache. m->att receives the bf16 rows.
+static int kv8_attention(ditch_cuda_model *m, Layer &L, int li, int n, bool prefill, float scale) {
+    const Config &c = m->cfg;
+    ditch_cuda_device *dev = m->dev;
+    cudaStream_t st = dev->stream;
+    const int hd = c.head_dim, qd = c.qd(), kvd = c.kvd(), W = c.qkv_width();
+    float *qkv = m->qkv.as<float>();
+    if (c.qk_norm)
+        DITCH_LAUNCH(dev, head_norms(qkv, n, c.heads, c.kv_heads, hd, L.q_norm.as<float>(), L.k_norm.as<float>(), c.eps, st));
+    auto rows32 = [&](int col, int heads) { return kv::Rows{qkv + col, W, hd, kv::kF32, heads, W % 4 == 0}; };
+    auto rows16 = [&](DevBuf &b, int heads) { return kv::Rows{b.ptr, (long long)heads * hd, hd, kv::kBf16, heads, 1}; };
+    kv::AppendParams a{};
+    a.c = kv8_cache(m, li);
+    a.b = kv::Batch{m->kv8_off.as<int>(), m->kv8_len.as<int>(), m->kv8_table.as<int>(), m->kv8_seqs, n, m->kv8_max_new,
+                    m->kv8_max_len, (m->kv_len + kKv8Page - 1) / kKv8Page};
+    a.r = kv::Rope{m->rope_cos.as<float>(), m->rope_sin.as<float>(), m->rope_len, hd / 2, 0};
+    a.q = rows32(0, c.heads);
+    a.k = rows32(qd, c.kv_heads);
+    a.v = rows32(qd + kvd, c.kv_heads);
+    a.qo = a.q;
+    if (prefill) {
+        DITCH_CUDA(m->kv8_q16.reserve((size_t)n * qd * 2));
+        DITCH_CUDA(m->kv8_k16.reserve((size_t)n * kvd * 2));
+        DITCH_CUDA(m->kv8_v16.reserve((size_t)n * kvd * 2));
+        a.qo = rows16(m->kv8_q16, c.heads);
+        a.ko = rows16(m->kv8_k16, c.kv_heads);
+        a.vo = rows16(m->kv8_v16, c.kv_heads);
+    }
+    a.status = dev->status;
+    DITCH_LAUNCH(dev, kv::append(a, st));
+    const kv::Rows out{m->att.ptr, qd, hd, kv::kBf16, c.heads, 1};
+    const int window = (int)m->kv8_window, sinks = (int)m->kv8_sinks;
+    if (prefill) {
+        kv::WindowParams w{};
+        w.b = kv::Ragged{a.b.offsets, a.b.offsets, m->kv8_seqs, n, n, m->kv8_max_new, m->kv8_max_new};
+        w.q = a.qo;
+        w.k = a.ko;
+        w.v = a.vo;
+        w.out = out;
+        w.dim = hd;
+        w.scale = scale;
+        w.window = window;
+        w.sinks = sinks;
+        w.status = dev->status;
+        DITCH_LAUNCH(dev, kv::window_attention(w, dev->sms, st));
+        return DITCH_CUDA_OK;
+    }
+    kv::AttendParams t{};
+    t.c = a.c;
+    t.b = a.b;
+    t.q = a.q;
+    t.out = out;
+    t.scale = scale;
+    t.window = window;
+    t.sinks = sinks;
+    const size_t need = kv::attend_workspace(t.c, t.b, c.heads, dev->sms);
+    if (need > m->kv8_ws_zeroed) {
+        DITCH_CUDA(m->kv8_ws.reserve(need));
+        DITCH_CUDA(cudaMemsetAsync(m->kv8_ws.ptr, 0, need, st));
+        m->kv8_ws_zeroed = need;
+    }
+    t.ws = m->kv8_ws.ptr;
+    t.status = dev->status;
+    DITCH_LAUNCH(dev, kv::attend(t, dev->sms, st));
+    return DITCH_CUDA_OK;
+}
+
 int forward_batch(ditch_cuda_model *m, Batch &b, int nc, int nl, int mode) {
     const Config &c = m->cfg;
     ditch_cuda_device *dev = m->dev;
@@ -519,6 +627,8 @@ int forward_batch(ditch_cuda_model *m, Batch &b, int nc, int nl, int mode) {
         ap.tc = dev->attn_tc;
         if (mode == kFwdPrompts) {
             DITCH_LAUNCH(dev, attention_prefill(ap, st));
+        } else if (m->kv8_format >= 0) {
+            if ((s = kv8_attention(m, L, li, n, mode == kFwdPromptsCache, ap.scale))) return s;
         } else {
             // the cache of this layer; decode rows store their key and value
             // first, so each attends to its own key as well
@@ -1272,6 +1382,27 @@ int ditch_cuda_set_row_normalization(ditch_cuda_model *m, int mode, size_t lora_
     return DITCH_CUDA_OK;
 }
 
+int ditch_cuda_model_set_kv_cache(ditch_cuda_model *m, int format, size_t window, size_t sinks) {
+    clear_error();
+    REQUIRE(m, "null model");
+    REQUIRE(format == DITCH_KV_NONE || format == DITCH_KV_INT8 || format == DITCH_KV_FP8, "unknown cache format %d", format);
+    REQUIRE(window < (1u << 30) && sinks < (1u << 30), "window %zu or sinks %zu too large", window, sinks);
+    REQUIRE(sinks == 0 || window > 0, "sinks without a window");
+    REQUIRE(format != DITCH_KV_NONE || window == 0, "the f32 cache has no window");
+    std::lock_guard<std::mutex> lk(m->dev->mu);
+    const Config &c = m->cfg;
+    if (format != DITCH_KV_NONE && (c.head_dim % 16 || c.head_dim > 128 || m->split3 || c.ep_world > 1 || c.tp_world > 1)) {
+        set_error("the 8-bit cache takes head sizes that are multiples of 16 up to 128 (this model's: %d), on one GPU, "
+                  "without the f32 split mode",
+                  c.head_dim);
+        return DITCH_CUDA_UNSUPPORTED;
+    }
+    m->kv8_format = format;
+    m->kv8_window = window;
+    m->kv8_sinks = sinks;
+    return DITCH_CUDA_OK;
+}
+
 int ditch_cuda_generate(ditch_cuda_model *m, const uint32_t *tokens, const size_t *prompt_offsets, size_t n_prompts,
                         size_t max_new_tokens, const uint32_t *eos_ids, size_t n_eos, uint32_t *out_tokens,
                         size_t *out_counts) {
@@ -1302,9 +1433,21 @@ int ditch_cuda_generate(ditch_cuda_model *m, const uint32_t *tokens, const size_
             max_new_tokens, m->rope_len);
     // KvCache.initFor(model, prompts, longest + max_new + 1) (src/engine.zig:254-260)
     const size_t max_len = longest + max_new_tokens + 1;
-    const size_t cache_bytes = (size_t)c.n_layers * P * max_len * c.kvd() * 4;
-    DITCH_CUDA(m->kv_k.reserve(cache_bytes));
-    DITCH_CUDA(m->kv_v.reserve(cache_bytes));
+    const bool kv8 = m->kv8_format >= 0;
+    if (kv8) {
+        const size_t pages = P * ((max_len + kKv8Page - 1) / kKv8Page);
+        REQUIRE(pages < (1u << 30), "too many prompts for the cache's pages");
+        const size_t tokens = (size_t)c.n_layers * pages * kKv8Page;
+        m->kv8_pages = (int)pages;
+        DITCH_CUDA(m->kv8_k.reserve(tokens * c.kvd()));
+        DITCH_CUDA(m->kv8_v.reserve(tokens * c.kvd()));
+        DITCH_CUDA(m->kv8_ks.reserve(tokens / kKv8Block * c.kv_heads * 4));
+        DITCH_CUDA(m->kv8_vs.reserve(tokens / kKv8Block * c.kv_heads * 4));
+    } else {
+        const size_t cache_bytes = (size_t)c.n_layers * P * max_len * c.kvd() * 4;
+        DITCH_CUDA(m->kv_k.reserve(cache_bytes));
+        DITCH_CUDA(m->kv_v.reserve(cache_bytes));
+    }
     DITCH_CUDA(m->gen_next.reserve(P * 4));
     m->kv_slots = (int)P;
     m->kv_len = (int)max_len;
@@ -1326,6 +1469,11 @@ int ditch_cuda_generate(ditch_cuda_model *m, const uint32_t *tokens, const size_
         }
     DITCH_CUDA(upload_vec(b.row_b, rb, st));
     DITCH_CUDA(upload_vec(b.row_pos, rp, st));
+    if (kv8) {
+        std::vector<int> slots(P);
+        for (size_t p = 0; p < P; p++) slots[p] = (int)p;
+        if ((s = kv8_begin(m, b.h_len, b.h_len, slots))) return s;
+    }
     if ((s = forward_batch(m, b, 0, (int)P, kFwdPromptsCache))) return s;
     std::vector<uint32_t> next(P);
     DITCH_LAUNCH(dev, argmax_rows(m->logits.as<float>(), (int)P, V, m->gen_next.as<uint32_t>(), st));
@@ -1386,6 +1534,11 @@ int ditch_cuda_generate(ditch_cuda_model *m, const uint32_t *tokens, const size_
         DITCH_CUDA(upload_vec(b.row_b, rb, st));
         DITCH_CUDA(upload_vec(b.row_pos, rp, st));
         DITCH_CUDA(upload_vec(b.logit_rows, lr, st));
+        if (kv8) {
+            std::vector<int> lens(rp);
+            for (int &t : lens) t++;
+            if ((s = kv8_begin(m, std::vector<int>(n, 1), lens, rb))) return s;
+        }
         if ((s = forward_batch(m, b, 0, n, kFwdDecode))) return s;
         DITCH_LAUNCH(dev, argmax_rows(m->logits.as<float>(), n, V, m->gen_next.as<uint32_t>(), st));
         DITCH_CUDA(cudaMemcpyAsync(next.data(), m->gen_next.ptr, (size_t)n * 4, cudaMemcpyDeviceToHost, st));

@@ -160,6 +160,7 @@ SIGNATURES = {
     "ditch_cuda_kv_attention_workspace": (sz, [vp, vp, vp, sz]),
     "ditch_cuda_kv_attention": (C.c_int, [vp] * 5 + [C.c_float, sz, sz, vp, sz, vp]),
     "ditch_cuda_window_attention": (C.c_int, [vp, vp, sz, vp, vp, vp, vp, C.c_float, sz, sz, vp]),
+    "ditch_cuda_model_set_kv_cache": (C.c_int, [vp, C.c_int, sz, sz]),
     "ditch_cuda_weight_load": (C.c_int, [vp, C.POINTER(TensorDesc), C.POINTER(vp)]),
     "ditch_cuda_weight_free": (None, [vp]),
     "ditch_cuda_weight_format": (C.c_int, [vp]),
@@ -838,6 +839,12 @@ class Model:
         `seed` + the matrix's index)."""
         code = {"none": 0, "pre": 1, "full": 2}[mode]
         check(lib().ditch_cuda_set_row_normalization(self.h, code, int(lora_rank), int(seed)))
+
+    def set_kv_cache(self, format=None, window=0, sinks=0):
+        """The cache of generate: None (f32, the reference's layout), "int8" or
+        "fp8" (paged, 8 bits, optionally with a sliding window and sinks)."""
+        code = -1 if format is None else KvCache.FORMATS[format]
+        check(lib().ditch_cuda_model_set_kv_cache(self.h, code, int(window), int(sinks)))
 
     def generate(self, prompts, max_new_tokens, eos_ids=()):
         """Greedy generation (model.generate, src/model.zig:5359-5444): a list

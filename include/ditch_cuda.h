@@ -499,6 +499,19 @@ int ditch_cuda_window_attention(ditch_cuda_device *dev, const ditch_cuda_ragged 
                                 const ditch_cuda_rows *q, const ditch_cuda_rows *k, const ditch_cuda_rows *v,
                                 const ditch_cuda_rows *out, float scale, size_t window, size_t sinks, void *stream);
 
+/* The cache of ditch_cuda_generate: DITCH_KV_NONE (the default) keeps the f32
+ * cache of the reference's layout; DITCH_KV_INT8 and DITCH_KV_FP8 keep the
+ * paged 8-bit one (pages of 64 tokens, blocks of 16): a quarter of the bytes,
+ * so four times the prompts or the tokens, and of every decode step's reads.
+ * The prompts' own attention is then ditch_cuda_window_attention over their
+ * bf16 rows, decode steps append and read the cache; both see `window`
+ * tokens and the first `sinks` (window 0: all). Keys and values are rounded to
+ * 8 bits, so tokens can differ from the f32 cache's where the best logits are
+ * near one another. Head sizes that the cache takes, one GPU (no expert or
+ * tensor parallelism), not the f32 split mode. */
+#define DITCH_KV_NONE (-1)
+int ditch_cuda_model_set_kv_cache(ditch_cuda_model *m, int format, size_t window, size_t sinks);
+
 /* ---- one resident weight and its dequant-fused GEMM ----
  * The product behind `matmulT` (src/tensor.zig:1023-1045) for one weight
  * kept in HBM in its stored format: FP8 blocks, MXFP4 and INT4 groups of 64k
