@@ -34,9 +34,8 @@
 // whatever the sequences' lengths. A CTA's share may begin and end inside an
 // item: it leaves that item's sums (f32) in the workspace, and the CTA that
 // brings an item's last part adds the parts in order, so results do not
-// depend on timing. Many short items (kernel parameter solo) are instead taken
-// whole, one by each warp, which needs neither: no sums to add, no waiting for
-// other warps.
+// depend on timing. Short items are taken whole instead, one by each CTA,
+// where that is done sooner (ITEMS): no parts, no counting of sequences.
 #include <algorithm>
 
 #include "gemm.cuh"
@@ -161,9 +160,9 @@ struct Layout {
     static constexpr int kRing = kWarps * kDepth * kStage;
     static constexpr int kO = kWarps * 8 * NT * DP * 4;
     static constexpr int kQf16 = (SPLIT ? 2 : 1) * 8 * NT * (DP + 8) * 2, kQdigits = 3 * 8 * NT * (DP + 16);
-    static constexpr int kQ = ((kQf16 > kQdigits ? kQf16 : kQdigits) + 15) & ~15;  // of the CTA, or of each warp
+    static constexpr int kQ = ((kQf16 > kQdigits ? kQf16 : kQdigits) + 15) & ~15;
     static constexpr int kQAt = kRing > kO ? kRing : kO;
-    static constexpr int bytes(bool solo) { return 1024 + kQAt + (solo ? kWarps : 1) * kQ; }
+    static constexpr int kBytes = 1024 + kQAt + kQ;
 };
 
 // A sequence's work: row tiles per head, and block slots of each (an upper
@@ -189,7 +188,7 @@ __device__ __forceinline__ Work work_of(const AttendParams &p, int group, int se
     return w;
 }
 
-template <int DP, int NT, bool SPLIT, bool FP8, bool SOLO>
+template <int DP, int NT, bool SPLIT, bool FP8, bool ITEMS>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     k_attend(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, AttendParams p) {
     using L = Layout<DP, NT, SPLIT>;
@@ -204,18 +203,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     constexpr int kPart = kRows * (DP + 2);   // floats of a part: sums, maxima, sums of weights
     extern __shared__ uint8_t smem_raw[];
     __shared__ Smem sm;
-    __shared__ float s_cs[(SOLO ? kWarps : 1) * kRows];
+    __shared__ float s_c[kRows];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    __half *s_q = reinterpret_cast<__half *>(base + L::kQAt + (SOLO ? warp * L::kQ : 0));
-    float *s_c = s_cs + (SOLO ? warp * kRows : 0);
-    // an item's warps: all of the CTA's, or this one
-    constexpr int kTeam = SOLO ? 1 : kWarps;
-    const int me = SOLO ? 0 : warp;
-    auto team_sync = [&]() {
-        if (SOLO) __syncwarp();
-        else __syncthreads();
-    };
+    __half *s_q = reinterpret_cast<__half *>(base + L::kQAt);
     const int group = p.q.heads / p.c.heads;
     int8_t *s_d = reinterpret_cast<int8_t *>(s_q);
     uint8_t *ring = base + warp * (kDepth * L::kStage);
@@ -235,54 +226,54 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     int seq = 0, item = 0, off = 0;
     Work work;
     long long pos = 0, end = 1, per = 1;
-    if constexpr (!SOLO) {
-    // ---- this CTA's share of the block slots: [pos, end) ----
-    const int chunk = (p.b.n_seqs + kThreads - 1) / kThreads;  // sequences a thread counts
-    const int c_lo = min(tid * chunk, p.b.n_seqs), c_hi = min(c_lo + chunk, p.b.n_seqs);
-    long long mine = 0;
-    for (int x = c_lo; x < c_hi; x++) {
-        const Work w = work_of<kRows>(p, group, x);
-        mine += static_cast<long long>(w.tiles) * w.slots * p.c.heads;
-    }
-    long long upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
-    }
-    if (lane == 31) sm.sums[warp] = upto;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-        if (w < warp) upto += sm.sums[w];
-        total += sm.sums[w];
-    }
-    per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinBlocks));
-    pos = per * blockIdx.x;
-    end = min(total, pos + per);
-    if (pos >= end) return;
-    if (upto - mine <= pos && pos < upto) {
-        long long at = upto - mine;
-        int x = c_lo;
-        for (;; x++) {
+    if constexpr (!ITEMS) {
+        // ---- this CTA's share of the block slots: [pos, end) ----
+        const int chunk = (p.b.n_seqs + kThreads - 1) / kThreads;  // sequences a thread counts
+        const int c_lo = min(tid * chunk, p.b.n_seqs), c_hi = min(c_lo + chunk, p.b.n_seqs);
+        long long mine = 0;
+        for (int x = c_lo; x < c_hi; x++) {
             const Work w = work_of<kRows>(p, group, x);
-            const long long n = static_cast<long long>(w.tiles) * w.slots * p.c.heads;
-            if (pos < at + n) break;
-            at += n;
+            mine += static_cast<long long>(w.tiles) * w.slots * p.c.heads;
         }
-        sm.seq = x;
-        sm.at = at;
-    }
-    __syncthreads();
-    seq = sm.seq;
-    work = work_of<kRows>(p, group, seq);
-    item = static_cast<int>((pos - sm.at) / work.slots);  // of the sequence: head * tiles + tile
-    off = static_cast<int>(pos - sm.at - static_cast<long long>(item) * work.slots);
-    } else {
-        // items are (sequence, head), dealt out to the warps
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane == 31) sm.sums[warp] = upto;
         __syncthreads();
-        pos = blockIdx.x + static_cast<long long>(gridDim.x) * warp;
+        long long total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            if (w < warp) upto += sm.sums[w];
+            total += sm.sums[w];
+        }
+        per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinBlocks));
+        pos = per * blockIdx.x;
+        end = min(total, pos + per);
+        if (pos >= end) return;
+        if (upto - mine <= pos && pos < upto) {
+            long long at = upto - mine;
+            int x = c_lo;
+            for (;; x++) {
+                const Work w = work_of<kRows>(p, group, x);
+                const long long n = static_cast<long long>(w.tiles) * w.slots * p.c.heads;
+                if (pos < at + n) break;
+                at += n;
+            }
+            sm.seq = x;
+            sm.at = at;
+        }
+        __syncthreads();
+        seq = sm.seq;
+        work = work_of<kRows>(p, group, seq);
+        item = static_cast<int>((pos - sm.at) / work.slots);  // of the sequence: head * tiles + tile
+        off = static_cast<int>(pos - sm.at - static_cast<long long>(item) * work.slots);
+    } else {
+        // items are (sequence, head), dealt out to the CTAs
+        __syncthreads();
+        pos = blockIdx.x;
         end = static_cast<long long>(p.b.n_seqs) * p.c.heads;
     }
 
@@ -292,19 +283,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     bool dead = false;   // a wait ran out
 
     while (pos < end) {
-        if constexpr (SOLO) {
+        if constexpr (ITEMS) {
             seq = static_cast<int>(pos / p.c.heads);
             item = static_cast<int>(pos - static_cast<long long>(seq) * p.c.heads);
             work = work_of<kRows>(p, group, seq);
             if (work.slots == 0) {
-                pos += static_cast<long long>(gridDim.x) * kWarps;
+                pos += gridDim.x;
                 continue;
             }
         }
         const Span a = work.a;
-        const int n_slots = SOLO ? work.slots : static_cast<int>(min(static_cast<long long>(work.slots - off), end - pos));
-        const int head = SOLO || work.tiles == 1 ? item : item / work.tiles, tile = item - head * work.tiles;
-        const int rows = a.n * group, r0 = SOLO ? 0 : tile * kRows, n_rows = min(kRows, rows - r0), first = a.len - a.n;
+        const int n_slots = ITEMS ? work.slots : static_cast<int>(min(static_cast<long long>(work.slots - off), end - pos));
+        const int head = ITEMS || work.tiles == 1 ? item : item / work.tiles, tile = item - head * work.tiles;
+        const int rows = a.n * group, r0 = ITEMS ? 0 : tile * kRows, n_rows = min(kRows, rows - r0), first = a.len - a.n;
         // row r of the tile is query (skip + r) mod group of the tile's token t0 + (skip + r) / group
         const int t0 = r0 ? r0 / group : 0, skip = r0 - t0 * group;
         const float per_group = 1.0f / group;
@@ -315,12 +306,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
 
         // ---- Q rows into registers ----
         // (lane l has dimensions 4 l .. 4 l + 3)
-        constexpr int kMine = kRows / kTeam;
+        constexpr int kMine = kRows / kWarps;
         float4 qx[kMine];
         const int d4 = 4 * lane;
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
-            const int r = me + kTeam * i, tok = tok_of(r);
+            const int r = warp + kWarps * i, tok = tok_of(r);
             const long long at = (a.row0 + t0 + tok) * p.q.ts + (head * group + skip + r - tok * group) * p.q.hs;
             qx[i] = r < n_rows && d4 < p.c.dim ? load4(p.q, at + d4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
@@ -332,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         };
         auto look_up = [&](int from) {
             Look k;
-            const int x = b_lo + 2 * (me + kTeam * (from + (lane >> 1))) + (lane & 1);
+            const int x = b_lo + 2 * (warp + kWarps * (from + (lane >> 1))) + (lane & 1);
             const int tok = range.token(x, kBlk);
             k.page = x < b_hi ? page_of(p.c, p.b, seq, tok, p.status) : -1;
             k.sk = k.sv = 0.0f;
@@ -361,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 page[h] = __shfl_sync(0xffffffffu, look.page, 2 * (i - ahead) + h);
-                u.tok[h] = page[h] < 0 ? -1 : range.token(b_lo + 2 * (me + kTeam * i) + h, kBlk);
+                u.tok[h] = page[h] < 0 ? -1 : range.token(b_lo + 2 * (warp + kWarps * i) + h, kBlk);
             }
             const int n = (page[0] >= 0) + (page[1] >= 0);
             if (n && lane == 0) {
@@ -391,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         scales(1, u1);
 #pragma unroll
         for (int i = 0; i < kMine; i++) {  // each row by a power of two to below 2
-            const int r = me + kTeam * i;
+            const int r = warp + kWarps * i;
             const float x[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
             uint32_t top = 0;
 #pragma unroll
@@ -428,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                 for (int d = 0; d < 3; d++) *reinterpret_cast<uint32_t *>(s_d + (d * kRows + r) * kQd + d4) = digit[d];
             }
         }
-        team_sync();
+        __syncthreads();
 
         float c_row[NT][2];
         int top_key[NT][2], low_key[NT][2];
@@ -669,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             }
         };
 
-        const int n_pairs = (b_hi - b_lo + 1) / 2, n_steps = me < n_pairs ? (n_pairs - me + kTeam - 1) / kTeam : 0;
+        const int n_pairs = (b_hi - b_lo + 1) / 2, n_steps = warp < n_pairs ? (n_pairs - warp + kWarps - 1) / kWarps : 0;
 #pragma unroll 1
         for (int i = 0; i < n_steps; i++) {
             use(st, u0);
@@ -705,25 +696,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                 store1(p.out, at + 3, v.w);
             }
         };
-        if constexpr (SOLO) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int r = 8 * n + 2 * t + e;
-                    if (r >= n_rows) continue;
-                    const float inv = m[n][e] == -INFINITY ? 0.0f : 1.0f / l[n][e];
-#pragma unroll
-                    for (int j = 0; j < kMt; j += 2) {
-                        const float2 a0 = unpack(o[n][j][0]), a1 = unpack(o[n][j][1]), a2 = unpack(o[n][j + 1][0]), a3 = unpack(o[n][j + 1][1]);
-                        put(r, g * (DP / 8) + 2 * j,
-                            e ? make_float4(a0.y * inv, a1.y * inv, a2.y * inv, a3.y * inv)
-                              : make_float4(a0.x * inv, a1.x * inv, a2.x * inv, a3.x * inv));
-                    }
-                }
-            pos += static_cast<long long>(gridDim.x) * kWarps;
-            __syncwarp();  // Q and the row factors have been read
-        } else {
         // ---- the warps' sums, in order ----
         if (g == 0) {
 #pragma unroll
@@ -745,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                 at[0] = make_float4(a0.x, a1.x, a2.x, a3.x);
                 at[DP / 4] = make_float4(a0.y, a1.y, a2.y, a3.y);
             }
-        const bool alone = off == 0 && n_slots == work.slots;
+        const bool alone = ITEMS || (off == 0 && n_slots == work.slots);
         const long long item_at = pos - off;
         const int c0 = static_cast<int>(item_at / per), c1 = static_cast<int>((item_at + work.slots - 1) / per);
         float *parts = reinterpret_cast<float *>(static_cast<uint8_t *>(p.ws) + kCounters * sizeof(int));
@@ -825,20 +797,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
         }
 
         // ---- on to the next item ----
-        pos += n_slots;
+        pos += ITEMS ? static_cast<int>(gridDim.x) : n_slots;
         off = 0;
         if (pos < end) {
-            item++;
-            if (item == work.tiles * p.c.heads) {
-                item = 0;
-                do {
-                    seq++;
-                    work = work_of<kRows>(p, group, seq);
-                } while (work.slots == 0);
+            if (!ITEMS) {
+                item++;
+                if (item == work.tiles * p.c.heads) {
+                    item = 0;
+                    do {
+                        seq++;
+                        work = work_of<kRows>(p, group, seq);
+                    } while (work.slots == 0);
+                }
             }
             fence_proxy_async_smem();  // the sums were read and written as plain memory, TMA writes there next
             __syncthreads();
-        }
         }
     }
 }
@@ -850,13 +823,16 @@ int tiles_of(const Cache &c, int max_new, int q_heads) {
     return rows <= 8 ? 1 : 2;
 }
 
-// Blocks a warp takes in the time that an item's beginning and end cost a CTA.
-constexpr int kItemCost = 10;
+// What the beginning and end of an item and of a part cost, in the time a warp
+// takes for a pair of blocks, about 1 us (measured: 1024 items of 11 blocks
+// 19.7 us whole, 33.5 us divided; 512 of 66 blocks 39 and 44 us; 8 of 250
+// blocks 32 and 21 us).
+constexpr long long kItemCost = 3, kPartCost = 8;
 
-template <int DP, int NT, bool SPLIT, bool SOLO>
+template <int DP, int NT, bool SPLIT, bool ITEMS>
 cudaError_t launch3(const AttendParams &p, const CUtensorMap &k_map, const CUtensorMap &v_map, long long grid, cudaStream_t s) {
-    constexpr int kBytes = Layout<DP, NT, SPLIT>::bytes(SOLO);
-    auto kernel = p.c.fp8 ? k_attend<DP, NT, SPLIT, true, SOLO> : k_attend<DP, NT, SPLIT, false, SOLO>;
+    constexpr int kBytes = Layout<DP, NT, SPLIT>::kBytes;
+    auto kernel = p.c.fp8 ? k_attend<DP, NT, SPLIT, true, ITEMS> : k_attend<DP, NT, SPLIT, false, ITEMS>;
     static SmemOptIn opt_in[2];
     const cudaError_t e = opt_in[p.c.fp8].set(reinterpret_cast<const void *>(kernel), kBytes);
     if (e != cudaSuccess) return e;
@@ -874,13 +850,12 @@ cudaError_t launch2(const AttendParams &p, int sms, cudaStream_t s) {
     long long seen = p.b.max_len;
     if (p.window) seen = std::min<long long>(seen, (long long)p.window + p.sinks + p.b.max_new + kBlk);
     const long long blocks = seen / kBlk + 2, wave = (long long)sms * ctas_per_sm<NT, SPLIT>();
-    if constexpr (NT == 1) {
-        // whole items to warps, when the longest would be done before an even
-        // division over CTAs, which pays for the beginning and end of each part
-        const long long solo = (items + kWarps * wave - 1) / (kWarps * wave) * blocks;
-        const long long even = items * blocks / (kWarps * wave) + kItemCost * (items / wave + 2);
-        if (solo <= even) return launch3<DP, NT, SPLIT, true>(p, k_map, v_map, std::min(wave, items), s);
-    }
+    // the longest item's pairs decide how long whole items take; an even
+    // division over CTAs pays for the beginning and end of each part
+    const long long pairs = (blocks + 1) / 2;
+    const long long whole = (items + wave - 1) / wave * ((pairs + kWarps - 1) / kWarps + kItemCost);
+    const long long even = items * pairs / (kWarps * wave) + kPartCost * (items / wave + 2);
+    if (tiles == 1 && whole <= even) return launch3<DP, NT, SPLIT, true>(p, k_map, v_map, std::min(wave, items), s);
     const long long most = std::min<long long>(items * ((blocks + kMinBlocks - 1) / kMinBlocks), kCounters);
     return launch3<DP, NT, SPLIT, false>(p, k_map, v_map, std::min(wave, most), s);
 }

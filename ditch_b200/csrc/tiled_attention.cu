@@ -566,29 +566,29 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             static_assert(kScaleSlots * (kScaleKeys / 16) == 32, "a lane each");
             const int block = lane % (kScaleKeys / 16);
             for (int j = lane / (kScaleKeys / 16); j < n; j += kScaleSlots) {
-                    const int key = range.token(j, kTileKeys) + 16 * block, slot = j % kScaleSlots;
-                    float sk = 0.0f, sv = 0.0f;
-                    long long codes = -1;
-                    if (key <= p_hi) {
-                        const int page = page_of(c, p.paged.b, seq, key, p.status);
-                        sk = __uint_as_float(0x7fc00000u);  // no page: the row is computed again without it
-                        if (page >= 0) {
-                            const long long at = scale_at(c, page, kvh, key);
-                            codes = code_at(c, page, kvh, key);
-                            sk = __ldg(c.ks + at);
-                            sv = __ldg(c.vs + at);
-                        }
+                const int key = range.token(j, kTileKeys) + 16 * block, slot = j % kScaleSlots;
+                float sk = 0.0f, sv = 0.0f;
+                long long codes = -1;
+                if (key <= p_hi) {
+                    const int page = page_of(c, p.paged.b, seq, key, p.status);
+                    sk = __uint_as_float(0x7fc00000u);  // no page: the row is computed again without it
+                    if (page >= 0) {
+                        const long long at = scale_at(c, page, kvh, key);
+                        codes = code_at(c, page, kvh, key);
+                        sk = __ldg(c.ks + at);
+                        sv = __ldg(c.vs + at);
                     }
-                    // never 0: a hidden score of -inf stays one, a weight of 0 leaves the sum of weights whole
-                    float ratio = sv / v_top;
-                    if (!(ratio >= 0x1p-40f)) ratio = ratio != ratio && v_top != 0.0f ? ratio : 0x1p-40f;
-                    if (j >= kScaleSlots && !mbar_wait(&bars.scales_empty[slot], (j / kScaleSlots + 1) & 1, abort, status)) break;
-                    bars.codes[slot][block] = codes;
-                    bars.sk[slot][block] = sk == 0.0f ? 0x1p-100f : sk;
-                    bars.lv[slot][block] = log2f(ratio);
-                    bars.iv[slot][block] = 1.0f / ratio;
-                    mbar_arrive(&bars.scales_full[slot]);
                 }
+                // never 0: a hidden score of -inf stays one, a weight of 0 leaves the sum of weights whole
+                float ratio = sv / v_top;
+                if (!(ratio >= 0x1p-40f)) ratio = ratio != ratio && v_top != 0.0f ? ratio : 0x1p-40f;
+                if (j >= kScaleSlots && !mbar_wait(&bars.scales_empty[slot], (j / kScaleSlots + 1) & 1, abort, status)) break;
+                bars.codes[slot][block] = codes;
+                bars.sk[slot][block] = sk == 0.0f ? 0x1p-100f : sk;
+                bars.lv[slot][block] = log2f(ratio);
+                bars.iv[slot][block] = 1.0f / ratio;
+                mbar_arrive(&bars.scales_full[slot]);
+            }
         }
     } else if (warp == S::kLoader) {
         if (lane == 0 && n > 0) {
@@ -666,196 +666,196 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     } else if (warp < 4 * S::kTiles) {
         if (S::kTrade) take_registers<S::kSoftmaxRegs>();
         if ((warp >> 2) < tiles) {
-        // ---- softmax of tile t: this thread's row ----
-        const int t = warp >> 2, row = tid & 127;
-        const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t s_cols = tmem + lanes + 128 * t, o_at = tmem + lanes + 128 * (S::kTiles + t);
-        const int tok = row / tl.heads, head = row - tok * tl.heads;  // of the tile
-        const int i = i0 + t * tl.toks + tok, pos = first + i;
-        const bool valid = tok < tl.toks && i < sq.nq && chunk * tl.heads + head < group;
-        // the tile's rows: the tiles of keys that all of them see whole need no masks
-        const int t_lo = first + i0 + t * tl.toks, t_hi = min(t_lo + tl.toks, first + sq.nq) - 1;
-        float c = p.scale * kLog2e;
-        if (PAGED && n > 0) {
-            // Q to f16: the row by a power of two to below 2, which c makes good
-            const int h = kvh * group + chunk * tl.heads + head;
-            const long long at = (sq.q0 + i) * p.q.ts + h * p.q.hs;
-            uint32_t top = 0;
-            if (valid)
-                for (int d = 0; d < p.dim; d += 4) {
-                    const float4 x = load4(p.q, at + d);
-                    top = max(max(top, __float_as_uint(x.x) & 0x7fffffffu), __float_as_uint(x.y) & 0x7fffffffu);
-                    top = max(max(top, __float_as_uint(x.z) & 0x7fffffffu), __float_as_uint(x.w) & 0x7fffffffu);
+            // ---- softmax of tile t: this thread's row ----
+            const int t = warp >> 2, row = tid & 127;
+            const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+            const uint32_t s_cols = tmem + lanes + 128 * t, o_at = tmem + lanes + 128 * (S::kTiles + t);
+            const int tok = row / tl.heads, head = row - tok * tl.heads;  // of the tile
+            const int i = i0 + t * tl.toks + tok, pos = first + i;
+            const bool valid = tok < tl.toks && i < sq.nq && chunk * tl.heads + head < group;
+            // the tile's rows: the tiles of keys that all of them see whole need no masks
+            const int t_lo = first + i0 + t * tl.toks, t_hi = min(t_lo + tl.toks, first + sq.nq) - 1;
+            float c = p.scale * kLog2e;
+            if (PAGED && n > 0) {
+                // Q to f16: the row by a power of two to below 2, which c makes good
+                const int h = kvh * group + chunk * tl.heads + head;
+                const long long at = (sq.q0 + i) * p.q.ts + h * p.q.hs;
+                uint32_t top = 0;
+                if (valid)
+                    for (int d = 0; d < p.dim; d += 4) {
+                        const float4 x = load4(p.q, at + d);
+                        top = max(max(top, __float_as_uint(x.x) & 0x7fffffffu), __float_as_uint(x.y) & 0x7fffffffu);
+                        top = max(max(top, __float_as_uint(x.z) & 0x7fffffffu), __float_as_uint(x.w) & 0x7fffffffu);
+                    }
+                int e2 = static_cast<int>(top >> 23) - 127;
+                e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
+                const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
+                c *= __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+                uint8_t *dst = s_q + t * L::kQTile + row * 128;
+#pragma unroll
+                for (int d = 0; d < DP; d += 8) {
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+                    if (valid && d < p.dim) {
+                        x = load4(p.q, at + d);
+                        y = load4(p.q, at + d + 4);
+                    }
+                    *reinterpret_cast<uint4 *>(dst + (d >> 6) * L::kQHalf + ((((d & 63) >> 3) ^ (row & 7)) << 4)) =
+                        make_uint4(pack16<false>(x.x * down, x.y * down), pack16<false>(x.z * down, x.w * down),
+                                   pack16<false>(y.x * down, y.y * down), pack16<false>(y.z * down, y.w * down));
                 }
-            int e2 = static_cast<int>(top >> 23) - 127;
-            e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
-            c *= __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
-            uint8_t *dst = s_q + t * L::kQTile + row * 128;
-#pragma unroll
-            for (int d = 0; d < DP; d += 8) {
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
-                if (valid && d < p.dim) {
-                    x = load4(p.q, at + d);
-                    y = load4(p.q, at + d + 4);
-                }
-                *reinterpret_cast<uint4 *>(dst + (d >> 6) * L::kQHalf + ((((d & 63) >> 3) ^ (row & 7)) << 4)) =
-                    make_uint4(pack16<false>(x.x * down, x.y * down), pack16<false>(x.z * down, x.w * down),
-                               pack16<false>(y.x * down, y.y * down), pack16<false>(y.z * down, y.w * down));
+                fence_proxy_async_smem();
+                mbar_arrive(&bars.q_full);
             }
-            fence_proxy_async_smem();
-            mbar_arrive(&bars.q_full);
-        }
-        float m = -INFINITY, l = 0.0f;  // m: the reference maximum of score * c, in base 2
-        bool ok = true;
-        for (int j = 0; j < n; j++) {
-            const uint32_t s_at = s_cols + kTileKeys * (j % kBuffers);
-            if (!mbar_wait(&bars.s_full[t][j % kBuffers], (j / kBuffers) & 1, abort, status)) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            uint32_t s[kTileKeys];
-#pragma unroll
-            for (int b = 0; b < kTileKeys; b += 32) tmem_ld32_start(s_at + b, s + b);
-            tmem_ld_wait();
-            const int k0 = range.token(j, kTileKeys);
-            if (k0 + kTileKeys - 1 > t_lo || (p.window && k0 <= t_hi - p.window)) {
-                const int hi = pos - k0, lo = p.window ? hi - p.window + 1 : 0, sink = p.sinks - k0;
-#pragma unroll
-                for (int b = 0; b < kTileKeys; b++)
-                    if (b > hi || (b < lo && b >= sink)) s[b] = 0xff800000u;
-            }
-            float f[kTileKeys / 16];  // factor of the scores of 16 keys
-            if (PAGED) {
-                if (!mbar_wait(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, abort, status)) {
+            float m = -INFINITY, l = 0.0f;  // m: the reference maximum of score * c, in base 2
+            bool ok = true;
+            for (int j = 0; j < n; j++) {
+                const uint32_t s_at = s_cols + kTileKeys * (j % kBuffers);
+                if (!mbar_wait(&bars.s_full[t][j % kBuffers], (j / kBuffers) & 1, abort, status)) {
                     ok = false;
                     break;
                 }
+                tc_fence_after();
+                uint32_t s[kTileKeys];
 #pragma unroll
-                for (int b = 0; b < kTileKeys / 16; b++) f[b] = c * bars.sk[j % kScaleSlots][b];
-            }
-            float mx = -INFINITY;
-            if (PAGED) {
+                for (int b = 0; b < kTileKeys; b += 32) tmem_ld32_start(s_at + b, s + b);
+                tmem_ld_wait();
+                const int k0 = range.token(j, kTileKeys);
+                if (k0 + kTileKeys - 1 > t_lo || (p.window && k0 <= t_hi - p.window)) {
+                    const int hi = pos - k0, lo = p.window ? hi - p.window + 1 : 0, sink = p.sinks - k0;
 #pragma unroll
-                for (int b = 0; b < kTileKeys / 16; b++) {
-                    float x = __uint_as_float(s[16 * b]), y = __uint_as_float(s[16 * b + 1]);
-#pragma unroll
-                    for (int e = 2; e < 14; e += 4) {
-                        x = max3(x, __uint_as_float(s[16 * b + e]), __uint_as_float(s[16 * b + e + 1]));
-                        y = max3(y, __uint_as_float(s[16 * b + e + 2]), __uint_as_float(s[16 * b + e + 3]));
-                    }
-                    x = max3(x, __uint_as_float(s[16 * b + 14]), __uint_as_float(s[16 * b + 15]));
-                    mx = fmaxf(mx, fmaxf(x, y) * f[b]);
+                    for (int b = 0; b < kTileKeys; b++)
+                        if (b > hi || (b < lo && b >= sink)) s[b] = 0xff800000u;
                 }
-            } else {
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int b = 0; b < kTileKeys; b += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) top[e] = max3(top[e], __uint_as_float(s[b + e]), __uint_as_float(s[b + 4 + e]));
-                mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-            }
-            if (__any_sync(0xffffffffu, mx - m > kLazy)) {
-                const float to = fmaxf(m, mx);
-                const float keep = m == -INFINITY ? 0.0f : exp2f(m - to);
-                m = to;
-                l *= keep;
-                if (j > 0) {  // P.V(j - 1) of all tiles is in (P.V(j) waits for this row, so no later phase can be over)
-                    if (!mbar_wait(&bars.v_empty[(j - 1) % kStages], ((j - 1) / kStages) & 1, abort, status)) {
+                float f[kTileKeys / 16];  // factor of the scores of 16 keys
+                if (PAGED) {
+                    if (!mbar_wait(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, abort, status)) {
                         ok = false;
                         break;
                     }
-                    tc_fence_after();
 #pragma unroll
-                    for (int b = 0; b < DP; b += 32) {
-                        uint32_t o[32];
+                    for (int b = 0; b < kTileKeys / 16; b++) f[b] = c * bars.sk[j % kScaleSlots][b];
+                }
+                float mx = -INFINITY;
+                if (PAGED) {
+#pragma unroll
+                    for (int b = 0; b < kTileKeys / 16; b++) {
+                        float x = __uint_as_float(s[16 * b]), y = __uint_as_float(s[16 * b + 1]);
+#pragma unroll
+                        for (int e = 2; e < 14; e += 4) {
+                            x = max3(x, __uint_as_float(s[16 * b + e]), __uint_as_float(s[16 * b + e + 1]));
+                            y = max3(y, __uint_as_float(s[16 * b + e + 2]), __uint_as_float(s[16 * b + e + 3]));
+                        }
+                        x = max3(x, __uint_as_float(s[16 * b + 14]), __uint_as_float(s[16 * b + 15]));
+                        mx = fmaxf(mx, fmaxf(x, y) * f[b]);
+                    }
+                } else {
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int b = 0; b < kTileKeys; b += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) top[e] = max3(top[e], __uint_as_float(s[b + e]), __uint_as_float(s[b + 4 + e]));
+                    mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                }
+                if (__any_sync(0xffffffffu, mx - m > kLazy)) {
+                    const float to = fmaxf(m, mx);
+                    const float keep = m == -INFINITY ? 0.0f : exp2f(m - to);
+                    m = to;
+                    l *= keep;
+                    if (j > 0) {  // P.V(j - 1) of all tiles is in (P.V(j) waits for this row, so no later phase can be over)
+                        if (!mbar_wait(&bars.v_empty[(j - 1) % kStages], ((j - 1) / kStages) & 1, abort, status)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+#pragma unroll
+                        for (int b = 0; b < DP; b += 32) {
+                            uint32_t o[32];
+                            tmem_ld32_start(o_at + b, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st32(o_at + b, o);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.0f : -m;
+                f32x2 sum[2] = {0, 0};
+#pragma unroll
+                for (int b = 0; b < kTileKeys / 32; b++) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        const int at = 32 * b + 16 * q;
+                        const float fb = PAGED ? f[2 * b + q] : c, rb = PAGED ? ref + bars.lv[j % kScaleSlots][2 * b + q] : ref;
+                        const f32x2 f2 = pair_of(fb, fb), r2 = pair_of(rb, rb);
+                        f32x2 part[2] = {0, 0};
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const f32x2 x = fma2(pair_of(__uint_as_float(s[at + 2 * e]), __uint_as_float(s[at + 2 * e + 1])), f2, r2);
+                            const float2 v = floats_of(x), a = make_float2(exp2_sfu(v.x), exp2_sfu(v.y));
+                            f32x2 &to = PAGED ? part[e & 1] : sum[e & 1];
+                            to = add2(to, pair_of(a.x, a.y));
+                            w[8 * q + e] = pack16<BF16 && !PAGED>(a.x, a.y);
+                        }
+                        if (PAGED) {
+                            const float iv = bars.iv[j % kScaleSlots][2 * b + q];
+                            sum[q] = fma2(add2(part[0], part[1]), pair_of(iv, iv), sum[q]);
+                        }
+                    }
+                    if (kTileKeys == 128 && b == 2) {  // P.V of the first half may begin
+                        tmem_st_wait();
+                        tc_fence_before();
+                        mbar_arrive(&bars.p_full[t][0]);
+                    }
+                    tmem_st16_start(s_at + 16 * b, w);
+                }
+                const float2 s2 = floats_of(add2(sum[0], sum[1]));
+                l += s2.x + s2.y;
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&bars.p_full[t][kBuffers == 2 ? j & 1 : 1]);
+            }
+            // ---- out = O / l ----
+            if (ok && n > 0) {
+                ok = mbar_wait(&bars.o_full[t], 0, abort, status);
+                tc_fence_after();
+            }
+            if (ok) {
+                float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+                if (PAGED && n > 0) inv *= __uint_as_float(bars.v_top);
+                const long long at = (sq.q0 + i) * p.out.ts + (kvh * group + chunk * tl.heads + head) * p.out.hs;
+                bool odd = false;  // something is not finite
+#pragma unroll
+                for (int b = 0; b < DP; b += 32) {
+                    uint32_t o[32];
+                    if (n > 0) {
                         tmem_ld32_start(o_at + b, o);
                         tmem_ld_wait();
+                    }
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                        tmem_st32(o_at + b, o);
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * inv : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * inv : 0.0f;
+                            odd |= !(fabsf(v0) <= 3.4e38f && fabsf(v1) <= 3.4e38f);
+                            w[k] = pack16<BF16>(v0, v1);
+                        }
+                        if (valid && b + e < p.dim && p.out.vec)
+                            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out.p) + at + b + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        else if (valid && b + e < p.dim)
+#pragma unroll
+                            for (int k = 0; k < 8; k++) static_cast<uint16_t *>(p.out.p)[at + b + e + k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
                     }
                 }
-            }
-            const float ref = m == -INFINITY ? 0.0f : -m;
-            f32x2 sum[2] = {0, 0};
-#pragma unroll
-            for (int b = 0; b < kTileKeys / 32; b++) {
-                uint32_t w[16];
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    const int at = 32 * b + 16 * q;
-                    const float fb = PAGED ? f[2 * b + q] : c, rb = PAGED ? ref + bars.lv[j % kScaleSlots][2 * b + q] : ref;
-                    const f32x2 f2 = pair_of(fb, fb), r2 = pair_of(rb, rb);
-                    f32x2 part[2] = {0, 0};
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const f32x2 x = fma2(pair_of(__uint_as_float(s[at + 2 * e]), __uint_as_float(s[at + 2 * e + 1])), f2, r2);
-                        const float2 v = floats_of(x), a = make_float2(exp2_sfu(v.x), exp2_sfu(v.y));
-                        f32x2 &to = PAGED ? part[e & 1] : sum[e & 1];
-                        to = add2(to, pair_of(a.x, a.y));
-                        w[8 * q + e] = pack16<BF16 && !PAGED>(a.x, a.y);
-                    }
-                    if (PAGED) {
-                        const float iv = bars.iv[j % kScaleSlots][2 * b + q];
-                        sum[q] = fma2(add2(part[0], part[1]), pair_of(iv, iv), sum[q]);
-                    }
-                }
-                if (kTileKeys == 128 && b == 2) {  // P.V of the first half may begin
-                    tmem_st_wait();
-                    tc_fence_before();
-                    mbar_arrive(&bars.p_full[t][0]);
-                }
-                tmem_st16_start(s_at + 16 * b, w);
-            }
-            const float2 s2 = floats_of(add2(sum[0], sum[1]));
-            l += s2.x + s2.y;
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(&bars.p_full[t][kBuffers == 2 ? j & 1 : 1]);
-        }
-        // ---- out = O / l ----
-        if (ok && n > 0) {
-            ok = mbar_wait(&bars.o_full[t], 0, abort, status);
-            tc_fence_after();
-        }
-        if (ok) {
-            float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
-            if (PAGED && n > 0) inv *= __uint_as_float(bars.v_top);
-            const long long at = (sq.q0 + i) * p.out.ts + (kvh * group + chunk * tl.heads + head) * p.out.hs;
-            bool odd = false;  // something is not finite
-#pragma unroll
-            for (int b = 0; b < DP; b += 32) {
-                uint32_t o[32];
-                if (n > 0) {
-                    tmem_ld32_start(o_at + b, o);
-                    tmem_ld_wait();
-                }
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * inv : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * inv : 0.0f;
-                        odd |= !(fabsf(v0) <= 3.4e38f && fabsf(v1) <= 3.4e38f);
-                        w[k] = pack16<BF16>(v0, v1);
-                    }
-                    if (valid && b + e < p.dim && p.out.vec)
-                        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out.p) + at + b + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                    else if (valid && b + e < p.dim)
-#pragma unroll
-                        for (int k = 0; k < 8; k++) static_cast<uint16_t *>(p.out.p)[at + b + e + k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
+                uint32_t again = __ballot_sync(0xffffffffu, valid && odd);
+                while (again) {
+                    const int from = __ffs(again) - 1;
+                    again &= again - 1;
+                    const int r_i = __shfl_sync(0xffffffffu, i, from), r_head = __shfl_sync(0xffffffffu, head, from);
+                    compute_row<PAGED>(p, seq, sq.q0 + r_i, kvh * group + chunk * tl.heads + r_head, first + r_i, sq.k0, lane);
                 }
             }
-            uint32_t again = __ballot_sync(0xffffffffu, valid && odd);
-            while (again) {
-                const int from = __ffs(again) - 1;
-                again &= again - 1;
-                const int r_i = __shfl_sync(0xffffffffu, i, from), r_head = __shfl_sync(0xffffffffu, head, from);
-                compute_row<PAGED>(p, seq, sq.q0 + r_i, kvh * group + chunk * tl.heads + r_head, first + r_i, sq.k0, lane);
-            }
-        }
         }
     }
     tc_fence_before();
