@@ -315,12 +315,15 @@ __global__ void __launch_bounds__(kThreads) k_kv_append_step(AppendParams p, int
 // heads of at most 32 dimensions) of one scale's block for one kv head, of
 // keys or of values, in registers, so every row is read once: a block's
 // magnitudes meet by warp reduction and shared memory, then the same
-// registers are rounded to codes. (With 16 tokens a warp the registers left
-// 16 warps an SM: 8192 tokens took 89 us.) The CTAs after those of keys and
-// values rotate the query rows, a warp a few heads of one token, whose angles
-// are loaded once.
+// registers are rounded to codes. How many warps are on an SM decides the
+// time: 8192 tokens of 8 and 32 heads at f32 took 89 us at 16 tokens a warp
+// (16 warps), 72 us at 8 tokens and 24 warps; with 32 warps, at the price of a
+// few spills, the pass with its read is 2 % to 10 % shorter again. The CTAs
+// after those of keys and values rotate the query rows, a warp a few heads of
+// one token, whose angles are loaded once (a kernel of their own for them: 10
+// us more).
 template <int LPT>
-__global__ void __launch_bounds__(kThreads, 3) k_kv_append(AppendParams p, int kv_ctas, int ctas_per_slot, int parts) {
+__global__ void __launch_bounds__(kThreads, 4) k_kv_append(AppendParams p, int kv_ctas, int ctas_per_slot, int parts) {
     constexpr int kTpp = 32 / LPT;           // tokens of a pass
     constexpr int kTile = tile_tokens<LPT>(), kPasses = kTile / kTpp;
     __shared__ uint32_t s_top[kWarps];
