@@ -229,6 +229,7 @@ int ditch_cuda_window_attention(ditch_cuda_device *dev, const ditch_cuda_ragged 
     REQUIRE(seqs->n_seqs < kMaxCount && seqs->n_q < kMaxCount && seqs->n_kv < kMaxCount && seqs->max_q <= seqs->n_q &&
                 seqs->max_kv <= seqs->n_kv && seqs->n_q <= seqs->n_seqs * seqs->max_q,
             "window_attention: bad counts");
+    REQUIRE(seqs->n_seqs <= kv::kTiledSeqs, "window_attention: %zu sequences (at most %d)", seqs->n_seqs, kv::kTiledSeqs);
     REQUIRE(seqs->n_seqs == 0 || (seqs->q_offsets && seqs->kv_offsets), "window_attention: null offsets");
     REQUIRE(head_dim > 0, "window_attention: bad head size");
     if (head_dim % 8 || head_dim > 128) {

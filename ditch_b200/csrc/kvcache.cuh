@@ -86,6 +86,7 @@ cudaError_t read_back(const ReadParams &p, cudaStream_t s);
 size_t attend_workspace(const Cache &c, const Batch &b, int q_heads, int sms);
 cudaError_t attend(const AttendParams &p, int sms, cudaStream_t s);
 cudaError_t window_attention(const WindowParams &p, int sms, cudaStream_t s);
+constexpr int kTiledSeqs = 65535;  // sequences that the tiled kernel takes (a grid dimension)
 // The tiled (tcgen05) form of attend, for many rows; and what it costs.
 cudaError_t attend_tiled(const AttendParams &p, cudaStream_t s);
 double tiled_rounds(const AttendParams &p, int sms, long long seen);

@@ -24,9 +24,15 @@
 //     with N = 64 takes the 64 cycles of one with N = 128, for its A operand)
 //   64 keys, two row tiles: S(j + 1) is made while the softmax works on S(j);
 //     for the cache, whose codes then need half the registers on their way
-//     (512 tokens over 1000 to 8000: 238 us against 307 us)
+//     (4 sequences of 512 rows over 2500 to 6000: 238 us against 307 us)
 //   64 keys, one row tile, two CTAs an SM: short runs, where the beginning
 //     and end of a CTA count
+// Measured: 8192 rows of 64 heads under a window of 4096 in 717 us, 1150
+// TFLOP/s (0.69 of the burst peak of a plain product; 860 us in a loop that
+// meets the power limit); 4 x 512 rows over the cache in 213 us, 570 TFLOP/s.
+// Taking 25 to 50 % of the exponentials off the SFU (a polynomial on the FMA
+// pipe) changed nothing or cost 2 to 11 %.
+//
 // A row whose maximum has grown by more than 2^kLazy since its sums'
 // reference rescales its part of O in TMEM, once P.V(j - 1) is in; most never
 // do.
@@ -858,6 +864,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             }
         }
     }
+    // a wait that ran out: what this CTA has under way (loads, MMAs) gets 0.1 ms before its memory goes to another
+    if (*abort)
+        for (int i = 0; i < 100; i++) __nanosleep(1000);
     tc_fence_before();
     __syncthreads();
     if (warp == S::kIssuer) {
@@ -894,7 +903,7 @@ cudaError_t launch(const TiledParams &p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const int pairs = (p.max_q + S::kTiles * tl.toks - 1) / (S::kTiles * tl.toks);
     const long long nx = (long long)pairs * p.kv_heads * tl.chunks;
-    if (p.n_seqs > 65535 || nx > 0x7fffffffLL) return cudaErrorInvalidValue;
+    if (p.n_seqs > kTiledSeqs || nx > 0x7fffffffLL) return cudaErrorInvalidValue;
     k_tiled<DP, BF16, FP8, S><<<dim3((unsigned)nx, (unsigned)p.n_seqs), S::kThreads, Layout<DP, S>::kBytes, s>>>(q, k, v, p, tl, pairs);
     return cudaGetLastError();
 }

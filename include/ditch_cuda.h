@@ -484,7 +484,7 @@ int ditch_cuda_kv_attention(ditch_cuda_device *dev, const ditch_cuda_kv_cache *c
 
 /* Ragged sequences of contiguous rows: sequence b has query rows q_offsets[b]
  * .. q_offsets[b + 1] (the last of its tokens) and key / value rows
- * kv_offsets[b] .. kv_offsets[b + 1] (all of them). */
+ * kv_offsets[b] .. kv_offsets[b + 1] (all of them). At most 65,535 sequences. */
 typedef struct {
     size_t n_seqs, n_q, n_kv, max_q, max_kv;
     const int32_t *q_offsets, *kv_offsets; /* [n_seqs + 1] */

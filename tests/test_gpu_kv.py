@@ -182,6 +182,9 @@ APPENDS = [
     ("fp8", "f16", 6, 2, 112, 256, 16, [(19, 260), (300, 511)], 56, 0),
     ("int8", "f32", 2, 1, 16, 16, 16, [(5, 21), (31, 31)], 8, 0),
     ("int8", "bf16", 5, 5, 96, 32, 32, [(64, 70)], 0, 0),
+    # more sequences than one step of the search takes, with and without several new tokens
+    ("fp8", "bf16", 4, 2, 64, 16, 16, [(i % 4, 1 + i % 4 + i % 29) for i in range(150)], 32, 0),
+    ("int8", "f16", 4, 2, 32, 64, 32, [(i % 3 != 1, 1 + i % 90) for i in range(1100)], 16, 1),
 ]
 
 
@@ -317,6 +320,10 @@ ATTENDS = [
     ("fp8", "bf16", 2, 1, 32, 128, 64, [(1, 9000)], 0, 0),
     ("int8", "f32", 8, 1, 128, 64, 64, [(1, 12345), (1, 0x40)], 0, 0),
     ("int8", "bf16", 130, 1, 64, 64, 16, [(2, 100)], 1, 0),
+    # many sequences: divided evenly over the CTAs, whole to a CTA, and tiled
+    ("int8", "bf16", 8, 2, 64, 16, 16, [(1, 1 + 37 * i % 1500) for i in range(140)], 0, 0),
+    ("fp8", "f16", 4, 2, 128, 64, 16, [(i % 2, 2 + i % 60) for i in range(200)], 0, 0),
+    ("int8", "f16", 8, 2, 128, 32, 32, [(20 + i, 20 + i + 11 * i) for i in range(40)], 90, 3),
 ]
 
 
@@ -418,6 +425,7 @@ WINDOWS = [
     ("bf16", 8, 2, 128, [(300, 2500), (33, 70), (1, 1), (40, 2049)], 0, 0),
     ("f16", 14, 2, 64, [(95, 3001), (18, 18), (19, 500)], 2500, 4),
     ("bf16", 4, 4, 80, [(129, 129), (2100, 2100)], 0, 0),
+    ("bf16", 8, 2, 128, [(1 + i % 37, 1 + i % 37 + i % 5) for i in range(45)], 0, 0),
 ]
 
 
