@@ -558,10 +558,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             const Cache &c = p.paged.c;
             // the largest sv in sight (as bits: a NaN is above all)
             const int per_tile = kTileKeys >> c.block_shift;
+            // A tile can hold pages of which no row sees a key (before the window, after the sinks): they may be anyone's,
+            // or nobody's, and are not looked up. Their keys are hidden from all rows, whatever stands for them.
+            auto in_sight = [&](int key, int keys) { return key <= p_hi && (!p.window || key + keys > p_lo - p.window + 1 || key < p.sinks); };
             uint32_t top = 0;
             for (int b = lane; b < n * per_tile; b += 32) {
                 const int key = range.token(b / per_tile, kTileKeys) + ((b % per_tile) << c.block_shift);
-                if (key > p_hi) continue;
+                if (!in_sight(key, 1 << c.block_shift)) continue;
                 const int page = page_of(c, p.paged.b, seq, key, p.status);
                 if (page >= 0) top = max(top, __float_as_uint(__ldg(c.vs + scale_at(c, page, kvh, key))) & 0x7fffffffu);
             }
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 const int key = range.token(j, kTileKeys) + 16 * block, slot = j % kScaleSlots;
                 float sk = 0.0f, sv = 0.0f;
                 long long codes = -1;
-                if (key <= p_hi) {
+                if (in_sight(key, 16)) {
                     const int page = page_of(c, p.paged.b, seq, key, p.status);
                     sk = __uint_as_float(0x7fc00000u);  // no page: the row is computed again without it
                     if (page >= 0) {

@@ -1,0 +1,108 @@
+"""The paged 8-bit cache and windowed attention where scales, magnitudes, pages
+and offsets are out of the ordinary, against the definitions in f64.
+
+Tolerance of an output element of 16 bits, from the formats: its own rounding,
+u |out|, and the rounding of the softmax weights, u sum(p |v|) over the keys
+that the row sees, with u = 2^-11 (f16) or 2^-8 (bf16) and |out| at most that
+sum: 2 u sum(p max|v|) in all, and 5 % of it for the f32 sums, scores and
+exponentials. What a row does not see has no part in it.
+"""
+import numpy as np
+import pytest
+
+import ditch_b200
+from ditch_b200 import KvBatch, KvCache, Ragged, Rows
+from test_gpu_kv import DT, STEP, TOP, Pool, gen, ints, randn
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+def reference(q, k, v, scale, window, sinks):
+    """(out, sum of p max|v|) of f64 rows q [n, Hq, d] over k and v [len, Hkv, d], the queries the last of the tokens;
+    NaN for a row that sees a key or value that is not finite."""
+    n, hq, d = q.shape
+    length, hkv = k.shape[:2]
+    p, j = torch.arange(length - n, length, device=q.device), torch.arange(length, device=q.device)
+    ok = j[None] <= p[:, None]
+    if window:
+        ok &= (j[None] > p[:, None] - window) | (j[None] < sinks)
+    bad = ~(torch.isfinite(k).all(-1) & torch.isfinite(v).all(-1))
+    k, v = (torch.where(bad[..., None], torch.zeros_like(x), x) for x in (k, v))
+    out, bound = torch.zeros_like(q), torch.zeros_like(q[..., 0])
+    for h in range(hq):
+        kh = h // (hq // hkv)
+        s = (q[:, h] @ k[:, kh].T * scale).masked_fill(~ok, -torch.inf)
+        w = torch.softmax(s, -1)
+        out[:, h], bound[:, h] = w @ v[:, kh], w @ v[:, kh].abs().amax(-1)
+        out[(ok & bad[None, :, kh]).any(-1), h] = float("nan")
+    return out, bound
+
+
+def check(got, want, bound, dtype):
+    got = got.double()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine)
+    over = ((got - want).abs() / (2.1 * STEP[dtype] * bound + 1e-300)[..., None])[fine]
+    assert not over.numel() or float(over.max()) <= 1.0, float(over.max())
+
+
+def kernels_of(call):
+    """The names of the kernels that `call` runs."""
+    from torch.profiler import ProfilerActivity, profile
+
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA], acc_events=True) as p:
+        call()
+        torch.cuda.synchronize()
+    return [e.name for e in p.events()]
+
+
+def attend(pool, q, new, scale, window=0, sinks=0, kernel=None, out=None):
+    """The attention's rows; `kernel`: the kernel that the sizes are meant to reach."""
+    out = torch.zeros_like(q) if out is None else out
+    batch = pool.batch(new)
+    size = pool.cache.attention_workspace(batch, q.shape[1])
+    ws = torch.zeros(max(size, 16), dtype=torch.uint8, device="cuda")
+
+    def call():
+        pool.cache.attention(batch, Rows.of(q), Rows.of(out), scale, window=window, sinks=sinks, workspace=ws, workspace_bytes=size)
+
+    if kernel:
+        assert any(kernel in n for n in kernels_of(call))
+    else:
+        call()
+    torch.cuda.synchronize()
+    pool.cache.dev.synchronize()
+    return out
+
+
+def check_all(pool, q, out, new, scale, window, sinks, dtype, values=None):
+    at = 0
+    for b, (a, t) in enumerate(zip(new, pool.lens)):
+        k, v = (pool.values(w, b, t) for w in range(2)) if values is None else values[b]
+        check(out[at:at + a], *reference(q[at:at + a].double(), k, v, scale, window, sinks), dtype)
+        at += a
+
+
+# 8 sequences of 300 rows in groups of 4 on 8 heads: what the tiled kernel takes
+NEW = [300] * 8
+LENS = [900 + 61 * i for i in range(8)]
+
+
+@pytest.mark.parametrize("fmt,page,block", [("int8", 16, 16), ("fp8", 32, 16), ("int8", 32, 32)])
+def test_tiled_pages_out_of_sight(device, fmt, page, block):
+    """Tiles of 64 keys hold pages of which no row of the call sees a token:
+    freed entries there, and pages of another owner with scales that are not
+    finite, change nothing and are not reported."""
+    g = gen(1)
+    pool = Pool(device, g, fmt, LENS, 8, 128, page, block)
+    q = randn(g, sum(NEW), 32, 128).to(torch.bfloat16)
+    values = [[pool.values(w, b, t) for w in range(2)] for b, t in enumerate(LENS)]
+    others = torch.isnan(pool.scales[0]).flatten(1).any(1).nonzero().flatten().tolist()
+    for b, (a, t) in enumerate(zip(NEW, LENS)):
+        for x in range(-(-4 // page), (t - a - 256 + 1) // page):
+            pool.table[b, x] = (others[0], -1, 10 ** 6)[x % 3]
+    out = attend(pool, q, NEW, 128 ** -0.5, 256, 4, kernel="k_tiled")
+    check_all(pool, q, out, NEW, 128 ** -0.5, 256, 4, "bf16", values)
