@@ -72,8 +72,9 @@ struct RowState {
 #pragma unroll
         for (int i = 0; i < 4; i++) s = fmaf(q[i], k[i], s);
         s = attn::warp_sum(s) * scale2;
-        const float top = fmaxf(m, s);
-        const float keep = top == -INFINITY ? 1.0f : exp2f(m - top), w = top == -INFINITY ? 0.0f : exp2f(s - top);
+        const float top = fmaxf(m, s);  // (of a NaN and a number, the number)
+        const float keep = top == -INFINITY ? 1.0f : exp2f(m - top);
+        const float w = s == -INFINITY ? 0.0f : exp2f(s - top);  // a NaN score is a NaN weight, also while there is no maximum
         m = top;
         sum = sum * keep + w;
 #pragma unroll

@@ -106,3 +106,34 @@ def test_tiled_pages_out_of_sight(device, fmt, page, block):
             pool.table[b, x] = (others[0], -1, 10 ** 6)[x % 3]
     out = attend(pool, q, NEW, 128 ** -0.5, 256, 4, kernel="k_tiled")
     check_all(pool, q, out, NEW, 128 ** -0.5, 256, 4, "bf16", values)
+
+
+@pytest.mark.parametrize("layout", ["plain", "odd"])
+def test_window_attention_nan_key_first(device, layout):
+    """A NaN key that is the first, or the only one, that a row sees."""
+    g = gen(2)
+    pad = 0 if layout == "plain" else 3
+    q, k, v = (randn(g, 400, h * 64 + pad).to(torch.bfloat16)[:, :h * 64].unflatten(1, (h, 64)) for h in (4, 2, 2))
+    k[0, 1], k[150, 0] = float("nan"), float("nan")  # the first tokens of the two sequences
+    k[230, 1] = float("nan")
+    off = ints([0, 150, 400])
+    out = torch.zeros_like(q)
+    device.window_attention(Ragged(off, off, 2, 400, 400, 250, 250), Rows.of(q), Rows.of(k), Rows.of(v), Rows.of(out), 64, 0.125,
+                            window=70)
+    torch.cuda.synchronize()
+    device.synchronize()
+    for lo, hi in ((0, 150), (150, 400)):
+        check(out[lo:hi], *reference(*(x[lo:hi].double() for x in (q, k, v)), 0.125, 70, 0), "bf16")
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("window", [0, 700])
+def test_tiled_nan_key_scale_first(device, fmt, window):
+    """A NaN scale of the first keys that rows see, in the tiled kernel."""
+    g = gen(3)
+    pool = Pool(device, g, fmt, LENS, 8, 128, 16, 16)
+    pool.scales[0][int(pool.table[0, 0]), 3, 0] = float("nan")
+    pool.scales[0][int(pool.table[2, 20]), 5, 0] = float("nan")
+    q = randn(g, sum(NEW), 32, 128).to(torch.float16)
+    out = attend(pool, q, NEW, 128 ** -0.5, window, 0, kernel="k_tiled")
+    check_all(pool, q, out, NEW, 128 ** -0.5, window, 0, "f16")
