@@ -41,7 +41,10 @@
 // shared memory as TMA would; Q is brought into f16's range by a power of two
 // for each row. A block's scales work on the scores: sk in the factor that
 // multiplies them, sv, as a fraction of the largest in sight, in the exponent
-// of the weight that goes into P (taken out again of the sum of weights).
+// of the weight that goes into P (taken out again of the sum of weights). A
+// row's reference maximum is that of the scores with it, so the largest of the
+// weights that go into P is about 1, however small the values that the row
+// sees are beside others.
 //
 // What a row does not see has weight 0 in the product, and 0 times an
 // infinity or NaN is NaN: rows whose result is not finite are computed again
@@ -226,10 +229,10 @@ struct Bars {
     uint64_t s_full[2][2], p_full[2][2],  // P of the two tiles of 64 keys, or of the two halves of 128
          o_full[2], scales_full[kScaleSlots], scales_empty[kScaleSlots];
     // per 16 keys of a tile: the factor of scores, log2 of sv / the largest sv, its inverse
-    // and the offset of their codes (-1: none)
-    long long codes[kScaleSlots][kScaleKeys / 16];
+    // and the offsets of their K and V codes (-1: zeros)
+    long long codes[2][kScaleSlots][kScaleKeys / 16];
     float sk[kScaleSlots][kScaleKeys / 16], lv[kScaleSlots][kScaleKeys / 16], iv[kScaleSlots][kScaleKeys / 16];
-    uint32_t v_top;  // bits of the largest sv in sight
+    float v_top;  // the largest sv in sight
     uint32_t tmem;
     int abort;
 };
@@ -489,7 +492,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             mbar_init(&bars.scales_full[i], kScaleKeys / 16);
             mbar_init(&bars.scales_empty[i], 1);
         }
-        bars.v_top = 0;
         bars.abort = 0;
         fence_barrier_init();
         if (!PAGED && n > 0) load_first();
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
                 for (int i = 0; i < kMine; i++) {
                     const int at = i * (kConverters / kChunks);
-                    const long long off = bars.codes[slot][(r0 + at) >> 4];
+                    const long long off = bars.codes[u & 1][slot][(r0 + at) >> 4];
                     x[i] = at <= last && off >= 0 && in ? __ldg(reinterpret_cast<const uint4 *>(codes + off)) : make_uint4(0, 0, 0, 0);
                 }
             };
@@ -557,21 +559,28 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         if (n > 0) {
             // ---- pages and scales ----
             const Cache &c = p.paged.c;
-            // the largest sv in sight (as bits: a NaN is above all)
+            // the largest sv in sight and the smallest that is not 0 (as bits: a NaN is above all)
             const int per_tile = kTileKeys >> c.block_shift;
             // A tile can hold pages of which no row sees a key (before the window, after the sinks): they may be anyone's,
             // or nobody's, and are not looked up. Their keys are hidden from all rows, whatever stands for them.
             auto in_sight = [&](int key, int keys) { return key <= p_hi && (!p.window || key + keys > p_lo - p.window + 1 || key < p.sinks); };
-            uint32_t top = 0;
+            uint32_t top = 0, least = 0x7f800000u;
             for (int b = lane; b < n * per_tile; b += 32) {
                 const int key = range.token(b / per_tile, kTileKeys) + ((b % per_tile) << c.block_shift);
                 if (!in_sight(key, 1 << c.block_shift)) continue;
                 const int page = page_of(c, p.paged.b, seq, key, p.status);
-                if (page >= 0) top = max(top, __float_as_uint(__ldg(c.vs + scale_at(c, page, kvh, key))) & 0x7fffffffu);
+                const uint32_t sv = page >= 0 ? __float_as_uint(__ldg(c.vs + scale_at(c, page, kvh, key))) & 0x7fffffffu : 0u;
+                top = max(top, sv);
+                if (sv) least = min(least, sv);
             }
             top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) bars.v_top = top;
-            const float v_top = __uint_as_float(top);
+            least = __reduce_min_sync(0xffffffffu, least);
+            const float v_top = top ? __uint_as_float(top) : 1.0f;
+            if (lane == 0) bars.v_top = v_top;
+            // Ratios down to 2^-100 leave every weight that counts above 2^-126, where exp2 gives 0. Values that are all 0
+            // (their codes then count as 0) go by the smallest sv, so that their weights are in the others' reach.
+            constexpr float kLeast = 0x1p-100f;
+            const float nil = top ? fmaxf(__uint_as_float(least) / v_top, kLeast) : 1.0f;
             // a lane for each 16 keys of eight tiles, so that the loads' latencies are paid once for all of them
             static_assert(kScaleSlots * (kScaleKeys / 16) == 32, "a lane each");
             const int block = lane % (kScaleKeys / 16);
@@ -589,12 +598,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         sv = __ldg(c.vs + at);
                     }
                 }
-                // never 0: a hidden score of -inf stays one, a weight of 0 leaves the sum of weights whole
-                float ratio = sv / v_top;
-                if (!(ratio >= 0x1p-40f)) ratio = ratio != ratio && v_top != 0.0f ? ratio : 0x1p-40f;
+                float ratio = sv == 0.0f ? nil : sv / v_top;
+                if (!(ratio >= kLeast)) ratio = __uint_as_float(0x7fc00000u);  // the rows are computed again, one at a time
                 if (j >= kScaleSlots && !mbar_wait(&bars.scales_empty[slot], (j / kScaleSlots + 1) & 1, abort, status)) break;
-                bars.codes[slot][block] = codes;
-                bars.sk[slot][block] = sk == 0.0f ? 0x1p-100f : sk;
+                bars.codes[0][slot][block] = codes;
+                bars.codes[1][slot][block] = sv == 0.0f ? -1 : codes;
+                bars.sk[slot][block] = sk == 0.0f ? 0x1p-100f : sk;  // never 0: a hidden score of -inf stays one
                 bars.lv[slot][block] = log2f(ratio);
                 bars.iv[slot][block] = 1.0f / ratio;
                 mbar_arrive(&bars.scales_full[slot]);
@@ -716,7 +725,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 fence_proxy_async_smem();
                 mbar_arrive(&bars.q_full);
             }
-            float m = -INFINITY, l = 0.0f;  // m: the reference maximum of score * c, in base 2
+            float m = -INFINITY, l = 0.0f;  // m: the reference maximum of score * c (and log2 of sv's ratio), in base 2
             bool ok = true;
             for (int j = 0; j < n; j++) {
                 const uint32_t s_at = s_cols + kTileKeys * (j % kBuffers);
@@ -756,7 +765,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                             y = max3(y, __uint_as_float(s[16 * b + e + 2]), __uint_as_float(s[16 * b + e + 3]));
                         }
                         x = max3(x, __uint_as_float(s[16 * b + 14]), __uint_as_float(s[16 * b + 15]));
-                        mx = fmaxf(mx, fmaxf(x, y) * f[b]);
+                        mx = fmaxf(mx, fmaf(fmaxf(x, y), f[b], bars.lv[j % kScaleSlots][b]));
                     }
                 } else {
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -831,8 +840,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 tc_fence_after();
             }
             if (ok) {
-                float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
-                if (PAGED && n > 0) inv *= __uint_as_float(bars.v_top);
+                const float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+                const float unit = PAGED && n > 0 ? bars.v_top : 1.0f;
                 const long long at = (sq.q0 + i) * p.out.ts + (kvh * group + chunk * tl.heads + head) * p.out.hs;
                 bool odd = false;  // something is not finite
 #pragma unroll
@@ -847,7 +856,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         uint32_t w[4];
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            const float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * inv : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * inv : 0.0f;
+                            float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * inv : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * inv : 0.0f;
+                            if (PAGED) v0 *= unit, v1 *= unit;
                             odd |= !(fabsf(v0) <= 3.4e38f && fabsf(v1) <= 3.4e38f);
                             w[k] = pack16<BF16>(v0, v1);
                         }

@@ -137,3 +137,40 @@ def test_tiled_nan_key_scale_first(device, fmt, window):
     q = randn(g, sum(NEW), 32, 128).to(torch.float16)
     out = attend(pool, q, NEW, 128 ** -0.5, window, 0, kernel="k_tiled")
     check_all(pool, q, out, NEW, 128 ** -0.5, window, 0, "f16")
+
+
+@pytest.mark.parametrize("fmt,dtype,d,up,base", [
+    ("int8", "bf16", 128, 12, 0), ("fp8", "bf16", 64, 20, 0), ("int8", "bf16", 64, 30, 0), ("fp8", "bf16", 128, 60, 0),
+    ("int8", "bf16", 128, 70, -45), ("int8", "f16", 128, 14, -8), ("fp8", "f16", 64, 20, -10)])
+def test_tiled_uneven_value_scales(device, fmt, dtype, d, up, base):
+    """Blocks of values 2^up above the others: the rows that do not see them,
+    or give them next to no weight, keep their precision."""
+    g = gen(4)
+    pool = Pool(device, g, fmt, LENS, 8, d, 16, 16)
+    ks, vs = pool.scales
+    vs *= 2.0 ** base
+
+    def at(b, token):
+        return int(pool.table[b, token // 16])
+
+    vs[at(0, LENS[0] - 1)] *= 2.0 ** up    # the last tokens: most rows do not see them
+    vs[at(1, LENS[1] - 150)] *= 2.0 ** up  # amid the new tokens
+    vs[at(2, 17)] *= 2.0 ** up             # among the first tokens, with scores of -40
+    pool.codes[0][at(2, 17)] = pool.encode(torch.full((8, 16, d), -TOP[fmt], device="cuda"))
+    ks[at(2, 17)] = 1.0 / TOP[fmt]
+    q = randn(g, sum(NEW), 32, d).to(DT[dtype])
+    q[600:900] = (40 * d ** -0.5 + 0.1 * randn(g, 300, 32, d)).to(DT[dtype])
+    vs[at(3, 40)] = 0.0                    # values of 0, and very small ones
+    vs[at(4, 600)] *= 2.0 ** -50
+    out = attend(pool, q, NEW, d ** -0.5, kernel="k_tiled")
+    check_all(pool, q, out, NEW, d ** -0.5, 0, 0, dtype)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_tiled_values_all_zero(device, fmt):
+    g = gen(5)
+    pool = Pool(device, g, fmt, LENS, 8, 128, 16, 16)
+    pool.scales[1][:] = 0.0
+    q = randn(g, sum(NEW), 32, 128).to(torch.bfloat16)
+    out = attend(pool, q, NEW, 128 ** -0.5, out=torch.ones_like(q), kernel="k_tiled")
+    assert (out == 0).all()
