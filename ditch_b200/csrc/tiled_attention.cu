@@ -48,7 +48,8 @@
 //
 // What a row does not see has weight 0 in the product, and 0 times an
 // infinity or NaN is NaN: rows whose result is not finite are computed again
-// from the keys that they do see (compute_row).
+// from the keys that they do see (compute_row). A scale of the cache that is
+// not finite stays out of the products, and makes the rows that see it NaN.
 //
 // Contiguous rows that TMA cannot take (not 16-byte aligned) go by
 // k_window_rows, one warp for each row.
@@ -232,7 +233,8 @@ struct Bars {
     // and the offsets of their K and V codes (-1: zeros)
     long long codes[2][kScaleSlots][kScaleKeys / 16];
     float sk[kScaleSlots][kScaleKeys / 16], lv[kScaleSlots][kScaleKeys / 16], iv[kScaleSlots][kScaleKeys / 16];
-    float v_top;  // the largest sv in sight
+    uint32_t bad[kScaleSlots];  // a byte for each 16 keys: a scale is not finite
+    float v_top;                // the largest finite sv in sight
     uint32_t tmem;
     int abort;
 };
@@ -559,7 +561,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         if (n > 0) {
             // ---- pages and scales ----
             const Cache &c = p.paged.c;
-            // the largest sv in sight and the smallest that is not 0 (as bits: a NaN is above all)
+            // the largest finite sv in sight and the smallest that is not 0 (as bits)
             const int per_tile = kTileKeys >> c.block_shift;
             // A tile can hold pages of which no row sees a key (before the window, after the sinks): they may be anyone's,
             // or nobody's, and are not looked up. Their keys are hidden from all rows, whatever stands for them.
@@ -570,8 +572,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 if (!in_sight(key, 1 << c.block_shift)) continue;
                 const int page = page_of(c, p.paged.b, seq, key, p.status);
                 const uint32_t sv = page >= 0 ? __float_as_uint(__ldg(c.vs + scale_at(c, page, kvh, key))) & 0x7fffffffu : 0u;
-                top = max(top, sv);
-                if (sv) least = min(least, sv);
+                if (sv < 0x7f800000u) {
+                    top = max(top, sv);
+                    if (sv) least = min(least, sv);
+                }
             }
             top = __reduce_max_sync(0xffffffffu, top);
             least = __reduce_min_sync(0xffffffffu, least);
@@ -588,6 +592,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 const int key = range.token(j, kTileKeys) + 16 * block, slot = j % kScaleSlots;
                 float sk = 0.0f, sv = 0.0f;
                 long long codes = -1;
+                bool bad = false;
                 if (in_sight(key, 16)) {
                     const int page = page_of(c, p.paged.b, seq, key, p.status);
                     sk = __uint_as_float(0x7fc00000u);  // no page: the row is computed again without it
@@ -596,6 +601,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         codes = code_at(c, page, kvh, key);
                         sk = __ldg(c.ks + at);
                         sv = __ldg(c.vs + at);
+                        bad = !(fabsf(sk) <= 3.4e38f && fabsf(sv) <= 3.4e38f);
+                        if (bad) sk = sv = 0.0f;  // for the rows that do not see it
                     }
                 }
                 float ratio = sv == 0.0f ? nil : sv / v_top;
@@ -604,6 +611,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 bars.codes[0][slot][block] = codes;
                 bars.codes[1][slot][block] = sv == 0.0f ? -1 : codes;
                 bars.sk[slot][block] = sk == 0.0f ? 0x1p-100f : sk;  // never 0: a hidden score of -inf stays one
+                reinterpret_cast<uint8_t *>(&bars.bad[slot])[block] = bad;
                 bars.lv[slot][block] = log2f(ratio);
                 bars.iv[slot][block] = 1.0f / ratio;
                 mbar_arrive(&bars.scales_full[slot]);
@@ -726,7 +734,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 mbar_arrive(&bars.q_full);
             }
             float m = -INFINITY, l = 0.0f;  // m: the reference maximum of score * c (and log2 of sv's ratio), in base 2
-            bool ok = true;
+            bool ok = true, nan = false;  // nan: the row sees a scale that is not finite
             for (int j = 0; j < n; j++) {
                 const uint32_t s_at = s_cols + kTileKeys * (j % kBuffers);
                 if (!mbar_wait(&bars.s_full[t][j % kBuffers], (j / kBuffers) & 1, abort, status)) {
@@ -753,6 +761,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                     }
 #pragma unroll
                     for (int b = 0; b < kTileKeys / 16; b++) f[b] = c * bars.sk[j % kScaleSlots][b];
+                    if (const uint32_t bad = bars.bad[j % kScaleSlots])
+                        for (int b = 0; b < kTileKeys / 16; b++) {
+                            const int key = k0 + 16 * b;
+                            if (bad >> (8 * b) & 1) nan |= key <= pos && (!p.window || key + 15 > pos - p.window || key < p.sinks);
+                        }
                 }
                 float mx = -INFINITY;
                 if (PAGED) {
@@ -840,7 +853,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 tc_fence_after();
             }
             if (ok) {
-                const float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+                const float inv = nan ? __uint_as_float(0x7fc00000u) : m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
                 const float unit = PAGED && n > 0 ? bars.v_top : 1.0f;
                 const long long at = (sq.q0 + i) * p.out.ts + (kvh * group + chunk * tl.heads + head) * p.out.hs;
                 bool odd = false;  // something is not finite
@@ -868,7 +881,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                             for (int k = 0; k < 8; k++) static_cast<uint16_t *>(p.out.p)[at + b + e + k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
                     }
                 }
-                uint32_t again = __ballot_sync(0xffffffffu, valid && odd);
+                uint32_t again = __ballot_sync(0xffffffffu, valid && odd && !nan);
                 while (again) {
                     const int from = __ffs(again) - 1;
                     again &= again - 1;

@@ -174,3 +174,33 @@ def test_tiled_values_all_zero(device, fmt):
     q = randn(g, sum(NEW), 32, 128).to(torch.bfloat16)
     out = attend(pool, q, NEW, 128 ** -0.5, out=torch.ones_like(q), kernel="k_tiled")
     assert (out == 0).all()
+
+
+def test_tiled_value_scale_not_finite_is_not_slow(device):
+    """Rows that see a value scale that is not finite are NaN at once, and the
+    others are not computed again one by one."""
+    g = gen(6)
+    pool = Pool(device, g, "int8", LENS, 8, 128, 16, 16)
+    q = randn(g, sum(NEW), 32, 128).to(torch.bfloat16)
+
+    def time():
+        attend(pool, q, NEW, 128 ** -0.5)
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        batch = pool.batch(NEW)
+        size = pool.cache.attention_workspace(batch, 32)
+        ws = torch.zeros(max(size, 16), dtype=torch.uint8, device="cuda")
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        a.record()
+        pool.cache.attention(batch, Rows.of(q), Rows.of(out), 128 ** -0.5, workspace=ws, workspace_bytes=size)
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b)
+
+    clean = time()
+    pool.scales[1][int(pool.table[0, 45]), 2, 0] = float("nan")   # tokens 720..735: amid the new ones
+    pool.scales[1][int(pool.table[1, 3]), :, 0] = float("inf")    # seen by all rows of the sequence
+    pool.scales[0][int(pool.table[2, 5]), 7, 0] = float("nan")
+    out = attend(pool, q, NEW, 128 ** -0.5, kernel="k_tiled")
+    check_all(pool, q, out, NEW, 128 ** -0.5, 0, 0, "bf16")
+    assert time() < 5 * clean
