@@ -332,6 +332,10 @@ __global__ void __launch_bounds__(kThreads, 4) k_kv_append(AppendParams p, int k
     const bool rope = p.r.cos_t != nullptr;
 
     if (static_cast<int>(blockIdx.x) >= kv_ctas) {
+        if (blockIdx.x == gridDim.x - 1) {  // a sequence whose offsets decrease may have no slot to be reported from
+            for (int x = threadIdx.x; x < b.n_seqs; x += kThreads) span_of(b, p.c.page_shift, x, p.status);
+            return;
+        }
         query_rows<LPT>(p, (blockIdx.x - kv_ctas) * kWarps + warp, parts, lane);
         return;
     }
@@ -341,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_kv_append(AppendParams p, int k
     const int unit = (blockIdx.x - slot * ctas_per_slot) * (kWarps / wpu) + warp / wpu;
     const int seq = seq_of_slot(b, p.c.block_shift, slot, lane);
     const int nth = slot - ((__ldg(b.offsets + seq) >> p.c.block_shift) + 2 * seq);
+    if (nth < 0) return;  // rows before the first sequence's
     const Span a = span_of(b, p.c.page_shift, seq, p.status);
     const int start = a.len - a.n;
     const int lo = ((start >> p.c.block_shift) + nth) << p.c.block_shift;  // first token of the block
@@ -477,8 +482,8 @@ cudaError_t append(const AppendParams &p, cudaStream_t s) {
     const long long kv_ctas = step ? (step_units + per_cta - 1) / per_cta : slots * per_slot;
     const int heads_per_warp = 32 / lpt * kQPasses, parts = p.q.p ? (p.q.heads + heads_per_warp - 1) / heads_per_warp : 0;
     const long long q_units = (long long)p.b.n_tokens * parts, q_ctas = (q_units + kWarps - 1) / kWarps;
-    if (kv_ctas + q_ctas > 0x7fffffffLL || q_units > 0x7fffffffLL || step_units > 0x7fffffffLL) return cudaErrorInvalidValue;
-    const unsigned grid = (unsigned)(kv_ctas + q_ctas);
+    if (kv_ctas + q_ctas >= 0x7fffffffLL || q_units > 0x7fffffffLL || step_units > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const unsigned grid = (unsigned)(kv_ctas + q_ctas) + !step;  // several new tokens: one CTA looks at all sequences
     if (step) {
         if (lpt == 2) k_kv_append_step<2><<<grid, kThreads, 0, s>>>(p, (int)kv_ctas, parts);
         else if (lpt == 4) k_kv_append_step<4><<<grid, kThreads, 0, s>>>(p, (int)kv_ctas, parts);

@@ -204,3 +204,33 @@ def test_tiled_value_scale_not_finite_is_not_slow(device):
     out = attend(pool, q, NEW, 128 ** -0.5, kernel="k_tiled")
     check_all(pool, q, out, NEW, 128 ** -0.5, 0, 0, "bf16")
     assert time() < 5 * clean
+
+
+def test_append_offsets_that_begin_late_or_go_back(device):
+    """Rows before the first sequence are left alone; offsets that decrease are
+    reported. Several new tokens a sequence."""
+    g = gen(7)
+    lens, new = [70, 40, 33], [40, 8, 33]
+    pool = Pool(device, g, "int8", lens, 2, 64, 16, 16)
+    x = randn(g, 39 + sum(new), 2, 64)
+    n = len(x)
+    pool.cache.append(KvBatch(ints([39, 79, 87, 120]), ints(lens), pool.table, 3, n, 40, 70, pool.table.shape[1]), Rows.of(x), Rows.of(x))
+    got = [y.clone() for y in pool.codes + pool.scales]
+    torch.cuda.synchronize()
+    device.synchronize()
+    pool = Pool(device, gen(7), "int8", lens, 2, 64, 16, 16)
+    y = x[39:].contiguous()
+    pool.cache.append(pool.batch(new), Rows.of(y), Rows.of(y))
+    torch.cuda.synchronize()
+    device.synchronize()
+    for a, b in zip(got, pool.codes + pool.scales):
+        assert torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float()))
+    # the second sequence ends before it begins; the third overlaps the first
+    for first, offsets in ((0, [0, 40, 8, 48]), (60, [60, 100, 68, 108])):
+        x = randn(g, first + 48, 2, 64)
+        pool.cache.append(KvBatch(ints(offsets), ints([70, 40, 40]), pool.table, 3, len(x), 40, 70, pool.table.shape[1]), Rows.of(x),
+                          Rows.of(x))
+        torch.cuda.synchronize()
+        with pytest.raises(ditch_b200.DitchCudaError):
+            device.synchronize()
+    device.synchronize()
