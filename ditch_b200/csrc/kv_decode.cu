@@ -395,11 +395,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
             for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
             top = __reduce_max_sync(0xffffffffu, top);
             int e2 = static_cast<int>(top >> 23) - 127;
-            e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(120, e2));
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
+            e2 = top >= 0x7f800000u || top == 0 ? 0 : max(-120, min(FP8 ? 120 : 127, e2));  // (f16 holds 2^8, the digits no more than 2)
+            const float down = e2 == 127 ? 0x1p-127f : __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
             if (lane == 0) {
-                float c = p.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
-                if (!FP8) c = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : c * 0x1p-21f;
+                float c = p.scale * kLog2e * (FP8 ? 1.0f : 0x1p-21f) * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+                if (!FP8 && top >= 0x7f800000u) c = __uint_as_float(0x7fc00000u);
                 s_c[r] = c;
             }
             if (d4 >= DP) continue;

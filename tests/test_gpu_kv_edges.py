@@ -234,3 +234,25 @@ def test_append_offsets_that_begin_late_or_go_back(device):
         with pytest.raises(ditch_b200.DitchCudaError):
             device.synchronize()
     device.synchronize()
+
+
+@pytest.mark.parametrize("dtype,new", [("bf16", 1), ("f32", 1), ("bf16", 3), ("f32", 40)])
+@pytest.mark.parametrize("power", [121, 122, 125, 127])
+def test_int8_queries_near_the_largest_number(device, dtype, new, power):
+    """Queries of up to 2^power, over keys as small: ordinary scores."""
+    g = gen(8)
+    pool = Pool(device, g, "int8", [100, 130], 2, 64, 16, 16)
+    pool.scales[0] *= 2.0 ** -100
+    q = (randn(g, 2 * new, 8, 64) / 6).clamp(-0.999, 0.999)
+    q[:, :, 5] = 0.75
+    q = (q * 2.0 ** power).to(DT[dtype])
+    scale = 2.0 ** (100 - power + 2) / 8
+    out = attend(pool, q, [new, new], scale)
+    at = 0
+    for b, t in enumerate(pool.lens):
+        want, bound = reference(q[at:at + new].double(), pool.values(0, b, t), pool.values(1, b, t), scale, 0, 0)
+        if dtype == "f32":  # 22 bits of the queries, f32 sums: as the tests of ordinary queries
+            assert float((out[at:at + new].double() - want).abs().max()) <= 2e-5 * float(want.abs().max())
+        else:
+            check(out[at:at + new], want, bound, dtype)
+        at += new
