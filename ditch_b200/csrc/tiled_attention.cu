@@ -64,7 +64,8 @@ namespace kv {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 8.0f;  // a weight stays below 2^8
+constexpr float kLazy = 8.0f;   // a weight stays below 2^8 of the reference
+constexpr float kF16Up = 7.0f;  // and is taken times 2^7 where P is f16: its normal numbers then reach down to 2^-21
 constexpr int kRowWarps = 4;
 
 // ---- one row by one warp -----------------------------------------------------------
@@ -810,7 +811,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         }
                     }
                 }
-                const float ref = m == -INFINITY ? 0.0f : -m;
+                const float ref = m == -INFINITY ? 0.0f : (PAGED || !BF16 ? kF16Up : 0.0f) - m;
                 f32x2 sum[2] = {0, 0};
 #pragma unroll
                 for (int b = 0; b < kTileKeys / 32; b++) {

@@ -256,3 +256,54 @@ def test_int8_queries_near_the_largest_number(device, dtype, new, power):
         else:
             check(out[at:at + new], want, bound, dtype)
         at += new
+
+
+def sink_pool(device, fmt, lens, d):
+    """Token 5 of each sequence takes nearly all weight and has a value of 0; the other keys are 0."""
+    pool = Pool(device, gen(9), fmt, lens, 8, d, 16, 16)
+    values = (1 + 0.2 * randn(gen(10), pool.n, 8, 16, d)) * (TOP[fmt] / 3)
+    pool.codes[0][:] = pool.encode(torch.zeros_like(values))
+    pool.codes[1][:] = pool.encode(values)
+    pool.scales[0][:] = 1.0
+    pool.scales[1][:] = 1.0 / 16
+    first = pool.table[:, 0].long()
+    pool.codes[0][first, :, 5] = pool.encode(torch.ones(len(lens), 8, d, device="cuda"))
+    pool.codes[1][first, :, 5] = 0
+    return pool
+
+
+@pytest.mark.parametrize("fmt,dtype,bits", [
+    ("int8", "f32", 12.3), ("int8", "f32", 16.6), ("fp8", "f32", 12.3), ("fp8", "f32", 16.6), ("fp8", "f16", 19.7), ("fp8", "bf16", 20.5)])
+def test_small_weights_keep_their_bits(device, fmt, dtype, bits):
+    """A sink with nearly all weight and no value: what is left of the row is
+    made of weights of 2^-bits each, which keep their precision."""
+    d = 64
+    pool = sink_pool(device, fmt, [40, 33, 1000], d)
+    q = torch.full((3, 8, d), bits * float(np.log(2.0)) / d, device="cuda").to(DT[dtype])
+    out = attend(pool, q, [1, 1, 1], 1.0)
+    for b, t in enumerate(pool.lens):
+        want, bound = reference(q[b:b + 1].double(), pool.values(0, b, t), pool.values(1, b, t), 1.0, 0, 0)
+        if dtype == "f32":  # two halves of a product 2^-22, scores and exponents up to 17 in f32, sums of up to 1000 terms
+            assert float(((out[b:b + 1].double() - want).abs() / bound[..., None]).max()) <= 1e-5
+        else:
+            check(out[b:b + 1], want, bound, dtype)
+
+
+@pytest.mark.parametrize("fmt,dtype,bits", [("int8", "bf16", 20.5), ("fp8", "f16", 18.2)])
+def test_tiled_small_weights_keep_their_bits(device, fmt, dtype, bits):
+    pool = sink_pool(device, fmt, LENS, 128)
+    q = torch.full((sum(NEW), 32, 128), bits * float(np.log(2.0)) / 128, device="cuda").to(DT[dtype])
+    out = attend(pool, q, NEW, 1.0, kernel="k_tiled")
+    check_all(pool, q, out, NEW, 1.0, 0, 0, dtype)
+
+
+@pytest.mark.parametrize("length", [500, 2500])
+def test_window_attention_small_weights_keep_their_bits(device, length):
+    q = torch.full((length, 4, 64), 18.2 * float(np.log(2.0)) / 64, device="cuda").half()
+    k, v = torch.zeros(length, 2, 64, device="cuda").half(), (64 + 13 * randn(gen(11), length, 2, 64)).half()
+    k[5], v[5] = 1.0, 0.0  # (outputs of 2^-12 and more: f16's normal numbers)
+    off, out = ints([0, length]), torch.zeros_like(q)
+    device.window_attention(Ragged(off, off, 1, length, length, length, length), Rows.of(q), Rows.of(k), Rows.of(v), Rows.of(out), 64, 1.0)
+    torch.cuda.synchronize()
+    device.synchronize()
+    check(out, *reference(q.double(), k.double(), v.double(), 1.0, 0, 0), "f16")
