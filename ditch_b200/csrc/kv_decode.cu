@@ -213,7 +213,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
     constexpr int kDigits = FP8 ? 1 : 3;
     constexpr int kMt = DP / 16;       // tiles of 16 dimensions of O^T
     constexpr float kLazy = lazy(SPLIT);
-    constexpr bool kBiased = !FP8 && !SPLIT;  // V codes + 1152: see below
     constexpr int kPart = kRows * (DP + 2);   // floats of a part: sums, maxima, sums of weights
     extern __shared__ uint8_t smem_raw[];
     __shared__ Smem sm;
@@ -619,22 +618,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
                     }
                 }
             // ---- O^T += sv V^T . P^T ----
-            // Biased codes: the sums start at -1152 sum(P), from an MMA with the
-            // same rounded P, so the bias cancels within the block's f32 sum (an
-            // error of 2^-23 of 1152 sum(P), about 1e-5 of a typical block's).
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const uint32_t vt = tiles + (2 * u + 1) * L::kTile;
-                float zero[NT][4];
+                const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 f32x2 w[NT];
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) zero[n][e] = 0.0f;
-                    const uint32_t minus[4] = {0xe480e480u, 0xe480e480u, 0xe480e480u, 0xe480e480u};
-                    if (kBiased) mma_f16(zero[n], minus, pb[u][n][0], pb[u][n][1], zero[n]);
-                    w[n] = pack(sees[u][n][0] ? s.sv[u] : 0.0f, sees[u][n][1] ? s.sv[u] : 0.0f);
-                }
+                for (int n = 0; n < NT; n++) w[n] = pack(sees[u][n][0] ? s.sv[u] : 0.0f, sees[u][n][1] ? s.sv[u] : 0.0f);
                 // (an E4M3 NaN in memory past the sequence must not meet a weight of 0)
                 const int seen = whole[u] || !FP8 ? kBlk : s.tok[u] < 0 ? 0 : p_hi + 1 - s.tok[u];
                 uint32_t v[4][DP / 32];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9, dimensions (DP / 8) g ...
@@ -658,13 +648,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
 #pragma unroll
                     for (int half = 0; half < 2; half++) {  // dimensions (DP / 8) g + 4 i + 2 half, + 1
                         uint32_t f[4];
-                        value_pairs<FP8, kBiased>(v[0][i], v[1][i], half, f[0], f[1]);
-                        value_pairs<FP8, kBiased>(v[2][i], v[3][i], half, f[2], f[3]);
+                        value_pairs<FP8>(v[0][i], v[1][i], half, f[0], f[1]);
+                        value_pairs<FP8>(v[2][i], v[3][i], half, f[2], f[3]);
                         const int j = 2 * i + half;
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
                             float x[4];
-                            mma_f16(x, f, pb[u][n][0], pb[u][n][1], zero[n]);
+                            mma_f16(x, f, pb[u][n][0], pb[u][n][1], zero);
                             if (SPLIT) mma_f16(x, f, pl[u][SPLIT ? n : 0][0], pl[u][SPLIT ? n : 0][1], x);
                             fma2(o[n][j][0], pack(x[0], x[1]), w[n]);
                             fma2(o[n][j][1], pack(x[2], x[3]), w[n]);

@@ -307,3 +307,12 @@ def test_window_attention_small_weights_keep_their_bits(device, length):
     torch.cuda.synchronize()
     device.synchronize()
     check(out, *reference(q.double(), k.double(), v.double(), 1.0, 0, 0), "f16")
+
+
+@pytest.mark.parametrize("dtype,bits", [("f16", 19.7), ("bf16", 20.5), ("bf16", 17.1)])
+def test_int8_values_of_0_leave_nothing(device, dtype, bits):
+    """The same over int8 codes: a value of 0 with nearly all weight adds 0, also to f32 sums that are far smaller."""
+    pool = sink_pool(device, "int8", [40, 33, 1000], 64)
+    q = torch.full((3, 8, 64), bits * float(np.log(2.0)) / 64, device="cuda").to(DT[dtype])
+    out = attend(pool, q, [1, 1, 1], 1.0)
+    check_all(pool, q, out, [1, 1, 1], 1.0, 0, 0, dtype)
