@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<NT, SPLIT>())
 
         auto use = [&](int stage, const Under &s) {
             if ((s.tok[0] < 0 && s.tok[1] < 0) || dead) return;
-            if (!mbar_wait(&full[stage], (phase >> stage) & 1, &sm.abort, p.status)) {
+            if (!mbar_wait_warp(&full[stage], (phase >> stage) & 1, &sm.abort, p.status)) {
                 dead = true;
                 return;
             }

@@ -647,18 +647,18 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 }
                 __syncwarp();
             };
-            bool ok = mbar_wait(&bars.q_full, 0, abort, status);
+            bool ok = mbar_wait_warp(&bars.q_full, 0, abort, status);
             for (int j = 0; ok && j < min(kBuffers, n); j++) {
-                ok = mbar_wait(&bars.k_full[j], 0, abort, status);
+                ok = mbar_wait_warp(&bars.k_full[j], 0, abort, status);
                 if (!ok) break;
                 tc_fence_after();
                 for (int t = 0; t < tiles; t++) qk(t, j);
             }
             // what the products of step j read besides P: V(j) and K(j + kBuffers)
             auto operands = [&](int j) {
-                return mbar_wait(&bars.v_full[j % kStages], (j / kStages) & 1, abort, status) &&
+                return mbar_wait_warp(&bars.v_full[j % kStages], (j / kStages) & 1, abort, status) &&
                        (j + kBuffers >= n ||
-                        mbar_wait(&bars.k_full[(j + kBuffers) % kStages], ((j + kBuffers) / kStages) & 1, abort, status));
+                        mbar_wait_warp(&bars.k_full[(j + kBuffers) % kStages], ((j + kBuffers) / kStages) & 1, abort, status));
             };
             ok = ok && operands(0);
             for (int j = 0; ok && j < n; j++) {
@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
                     for (int half = 0; half < kTileKeys / 64; half++) {
                         if (!ok) break;
-                        ok = mbar_wait(&bars.p_full[t][kBuffers == 2 ? j & 1 : half], (j / kBuffers) & 1, abort, status);
+                        ok = mbar_wait_warp(&bars.p_full[t][kBuffers == 2 ? j & 1 : half], (j / kBuffers) & 1, abort, status);
                         if (!ok) break;
                         tc_fence_after();
                         if (leader) {
@@ -738,7 +738,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             bool ok = true, nan = false;  // nan: the row sees a scale that is not finite
             for (int j = 0; j < n; j++) {
                 const uint32_t s_at = s_cols + kTileKeys * (j % kBuffers);
-                if (!mbar_wait(&bars.s_full[t][j % kBuffers], (j / kBuffers) & 1, abort, status)) {
+                if (!mbar_wait_warp(&bars.s_full[t][j % kBuffers], (j / kBuffers) & 1, abort, status)) {
                     ok = false;
                     break;
                 }
@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 }
                 float f[kTileKeys / 16];  // factor of the scores of 16 keys
                 if (PAGED) {
-                    if (!mbar_wait(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, abort, status)) {
+                    if (!mbar_wait_warp(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, abort, status)) {
                         ok = false;
                         break;
                     }
@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                     m = to;
                     l *= keep;
                     if (j > 0) {  // P.V(j - 1) of all tiles is in (P.V(j) waits for this row, so no later phase can be over)
-                        if (!mbar_wait(&bars.v_empty[(j - 1) % kStages], ((j - 1) / kStages) & 1, abort, status)) {
+                        if (!mbar_wait_warp(&bars.v_empty[(j - 1) % kStages], ((j - 1) / kStages) & 1, abort, status)) {
                             ok = false;
                             break;
                         }
@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             }
             // ---- out = O / l ----
             if (ok && n > 0) {
-                ok = mbar_wait(&bars.o_full[t], 0, abort, status);
+                ok = mbar_wait_warp(&bars.o_full[t], 0, abort, status);
                 tc_fence_after();
             }
             if (ok) {
