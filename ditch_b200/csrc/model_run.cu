@@ -544,7 +544,6 @@ static int kv8_attention(ditch_cuda_model *m, Layer &L, int li, int n, bool pref
     const int window = (int)m->kv8_window, sinks = (int)m->kv8_sinks;
     if (prefill) {
         kv::WindowParams w{};
-        w.b = kv::Ragged{a.b.offsets, a.b.offsets, m->kv8_seqs, n, n, m->kv8_max_new, m->kv8_max_new};
         w.q = a.qo;
         w.k = a.ko;
         w.v = a.vo;
@@ -554,7 +553,10 @@ static int kv8_attention(ditch_cuda_model *m, Layer &L, int li, int n, bool pref
         w.window = window;
         w.sinks = sinks;
         w.status = dev->status;
-        DITCH_LAUNCH(dev, kv::window_attention(w, dev->sms, st));
+        for (int s0 = 0; s0 < m->kv8_seqs; s0 += kv::kTiledSeqs) {
+            w.b = kv::Ragged{a.b.offsets + s0, a.b.offsets + s0, std::min(kv::kTiledSeqs, m->kv8_seqs - s0), n, n, m->kv8_max_new, m->kv8_max_new};
+            DITCH_LAUNCH(dev, kv::window_attention(w, dev->sms, st));
+        }
         return DITCH_CUDA_OK;
     }
     kv::AttendParams t{};

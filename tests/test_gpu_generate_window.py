@@ -99,3 +99,20 @@ def test_windowed_generation(device, name, fmt, monkeypatch):
     n, exact = base.check_generation(WindowedModel(spec, f32, window, sinks), ps, got, 48)
     assert n == 48 * len(ps)
     print(f"{name} {fmt}: {exact} of {n} tokens with a clear maximum")
+
+
+@pytest.mark.gpu
+def test_more_prompts_than_one_windowed_prefill_takes(device, request):
+    """65,600 prompts, of which many are alike: those past one launch's 65,535
+    sequences get the tokens of their likes before it."""
+    spec, f32, tensors = make_model(995, n_layers=1, hidden=64, heads=1, kv_heads=1, head_dim=32, inter=64)
+    m = ditch_b200.Model(device, spec, tensors, max_seq=16)
+    device.set_deterministic(True)
+    request.addfinalizer(lambda: device.set_deterministic(False))
+    m.set_kv_cache("int8")
+    ps = [np.array([i % 64, 7], np.uint32) for i in range(65600)]
+    got = m.generate(ps, 3)
+    m.close()
+    assert len(got) == len(ps) and all(len(g) == 3 for g in got)
+    assert all(got[i] == got[i % 64] for i in range(len(ps)))
+    base.check_generation(OracleModel(spec, f32), ps[-8:], got[-8:], 3)
