@@ -789,7 +789,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                         for (int e = 0; e < 4; e++) top[e] = max3(top[e], __uint_as_float(s[b + e]), __uint_as_float(s[b + 4 + e]));
                     mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
                 }
-                if (__any_sync(0xffffffffu, mx - m > kLazy)) {
+                if (__any_sync(0xffffffffu, valid && mx - m > kLazy)) {  // (rows without a query hold what was there before)
                     const float to = fmaxf(m, mx);
                     const float keep = m == -INFINITY ? 0.0f : exp2f(m - to);
                     m = to;

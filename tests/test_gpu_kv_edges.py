@@ -316,3 +316,25 @@ def test_int8_values_of_0_leave_nothing(device, dtype, bits):
     q = torch.full((3, 8, 64), bits * float(np.log(2.0)) / 64, device="cuda").to(DT[dtype])
     out = attend(pool, q, [1, 1, 1], 1.0)
     check_all(pool, q, out, [1, 1, 1], 1.0, 0, 0, dtype)
+
+
+@pytest.mark.parametrize("dtype,length,window", [("f16", 700, 257), ("bf16", 2600, 0)])
+def test_window_attention_repeats_itself(device, dtype, length, window):
+    """Groups of 7 leave two rows of a tile of 128 without a query: what an
+    earlier kernel left in shared memory there changes no row."""
+    g = gen(12)
+
+    def run(q, k, v):
+        off, out = ints([0, len(q)]), torch.zeros_like(q)
+        device.window_attention(Ragged(off, off, 1, len(q), len(q), len(q), len(q)), Rows.of(q), Rows.of(k), Rows.of(v), Rows.of(out), 64,
+                                0.125, window=window)
+        torch.cuda.synchronize()
+        return out
+
+    q, k, v = (randn(g, length, h, 64).to(DT[dtype]) for h in (14, 2, 2))
+    k[:, :, ::9] *= 3
+    first = run(q, k, v)
+    for size in (1.0, 30.0, 300.0):
+        run(*((size * randn(g, length, h, 64)).to(DT[dtype]) for h in (16, 2, 2)))  # 8 queries a group: all rows
+        assert torch.equal(run(q, k, v), first)
+    device.synchronize()
