@@ -32,13 +32,16 @@
 // 2^-24 of f16's unit, whichever they are of).
 //
 // Measured: one row for each of 32 sequences of 4000 to 32000 tokens (1.01 GB
-// of E4M3 codes and scales) in 169 us, 5.97 TB/s, 0.91 of the copy bandwidth;
-// 64 sequences with 1028 tokens in sight (135 MB, int8) in 42 us, 3.2 TB/s,
-// where the beginning and end of each item show. With codes loaded straight
+// of E4M3 codes and scales) in 169 to 177 us on five boxes, 5.7 to 6.0 TB/s,
+// 0.87 to 0.91 of the copy bandwidth; 64 sequences with 1028 tokens in sight
+// (135 MB, int8) in 42 us, 3.2 TB/s, where the beginning and end of each item
+// show. With codes loaded straight
 // into registers instead of by TMA the first took 330 us.
 //
-// f32 rows: P (and Q over an E4M3 cache) is split into two f16 (22 bits), two
-// MMAs for one.
+// f32 out: P (and Q over an E4M3 cache) is split into two f16 (22 bits), two
+// MMAs for one. 16 bits out take both as one f16, f32 queries over an E4M3
+// cache as well: the split costs those 7 to 30 % (32 sequences of 16000 tokens
+// 175 us, with it 189; 128 of 1500 tokens on one head 17 and 22 us).
 //
 // The blocks of all work items (sequence, key / value head, row tile), one
 // item after another, are divided evenly over as many CTAs as the GPU holds,

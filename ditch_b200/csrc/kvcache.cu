@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_append_step(AppendParams p, int
 // few spills, the pass with its read is 2 % to 10 % shorter again. The CTAs
 // after those of keys and values rotate the query rows, a warp a few heads of
 // one token, whose angles are loaded once (a kernel of their own for them: 10
-// us more). 8192 tokens and the read of what was stored: 86 us, 4.7 TB/s.
+// us more). 8192 tokens and the read of what was stored: 87 us, 4.6 TB/s.
 template <int LPT>
 __global__ void __launch_bounds__(kThreads, 4) k_kv_append(AppendParams p, int kv_ctas, int ctas_per_slot, int parts) {
     constexpr int kTpp = 32 / LPT;           // tokens of a pass

@@ -20,16 +20,20 @@
 // P.V from there; V is taken as it lies, [token][dimension], as a transposed
 // (MN-major) B operand. Three shapes (Shape), by measurement at head size 128:
 //   128 keys, two row tiles a CTA: the least MMA time, for long runs of keys
-//     (8192 tokens, window 4096: 710 us, against 928 us with 64 keys: an MMA
-//     with N = 64 takes the 64 cycles of one with N = 128, for its A operand)
+//     (8192 tokens, window 4096: 838 us in a steady loop, which meets the
+//     power limit, and 744 us in bursts of three; with 64 keys 955 and 912 us,
+//     in one row tile a CTA 932 and 825 us: an MMA with N = 64 takes the 64
+//     cycles of one with N = 128, for its A operand)
 //   64 keys, two row tiles: S(j + 1) is made while the softmax works on S(j);
 //     for the cache, whose codes then need half the registers on their way
-//     (4 sequences of 512 rows over 2500 to 6000: 238 us against 307 us)
+//     (4 sequences of 512 rows over 2500 to 6000: 238 us against 307 us, when
+//     it was chosen)
 //   64 keys, one row tile, two CTAs an SM: short runs, where the beginning
 //     and end of a CTA count
-// Measured: 8192 rows of 64 heads under a window of 4096 in 717 us, 1150
-// TFLOP/s (0.69 of the burst peak of a plain product; 860 us in a loop that
-// meets the power limit); 4 x 512 rows over the cache in 213 us, 570 TFLOP/s.
+// Measured: 8192 rows of 64 heads under a window of 4096 in 729 to 744 us in
+// bursts, 1110 to 1130 TFLOP/s (0.66 to 0.68 of the burst peak of a plain
+// product), 830 to 859 us in a loop, 961 to 995 TFLOP/s (0.69 to 0.71 of the
+// sustained peak); 4 x 512 rows over the cache in 217 to 222 us, 550 TFLOP/s.
 // Taking 25 to 50 % of the exponentials off the SFU (a polynomial on the FMA
 // pipe) changed nothing or cost 2 to 11 %.
 //
@@ -39,7 +43,8 @@
 //
 // The cache's codes are f16 operands exactly (int8 and E4M3 fit), laid out in
 // shared memory as TMA would; Q is brought into f16's range by a power of two
-// for each row. A block's scales work on the scores: sk in the factor that
+// for each row and rounded to it (f32 queries to 11 bits: a second half would
+// take the shared memory of a row tile and a third of the MMAs again). A block's scales work on the scores: sk in the factor that
 // multiplies them, sv, as a fraction of the largest in sight, in the exponent
 // of the weight that goes into P (taken out again of the sum of weights). A
 // row's reference maximum is that of the scores with it, so the largest of the

@@ -395,7 +395,9 @@ int ditch_cuda_edit_weight_bf16_noalloc(void *w, size_t rows, size_t cols, const
  * returns without waiting and allocates nothing, so the calls can be captured
  * in a graph. What the kernels find wrong in device data (an offset, a length
  * or a page outside its bounds) is left out and sets the device's status
- * word: the next ditch_cuda_synchronize returns DITCH_CUDA_INVALID. */
+ * word. ditch_cuda_synchronize reports it (DITCH_CUDA_INVALID) and clears it,
+ * but waits for the library's own stream only: wait for `stream` first, or
+ * the report may come later, from another call that looks at the word. */
 #define DITCH_KV_INT8 0 /* codes -127..127 */
 #define DITCH_KV_FP8 1  /* codes E4M3 (largest 448; its NaN codes are never stored) */
 
@@ -417,7 +419,8 @@ typedef struct {
  * of the call's rows, the last ones of its lens[b] tokens (row i of it is at
  * position lens[b] - (offsets[b + 1] - offsets[b]) + i); token t of it lies in
  * page pages[b * max_pages + t / page_tokens]. Pages outside a window may hold
- * any number. The host's counts bound the device's: n_tokens rows, max_new
+ * any number. Offsets do not decrease; rows before offsets[0] belong to no
+ * sequence. The host's counts bound the device's: n_tokens rows, max_new
  * rows and max_len tokens of one sequence. */
 typedef struct {
     size_t n_seqs, n_tokens, max_new, max_len, max_pages;
@@ -469,13 +472,17 @@ int ditch_cuda_kv_read(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache,
  * out = sum softmax(scale * q . k) v, zero for a row that sees nothing. Query
  * head h reads kv head h / (heads / kv_heads). What a row does not see does
  * not change it (E4M3's NaN codes within its sequence excepted); a scale that
- * is not finite makes the rows that see its block not finite. f32 out is computed to f32
- * rounding, f16 and bf16 out with the softmax weights rounded to f16. The
- * workspace holds the partial sums of sequences split over the GPU: at least
- * ditch_cuda_kv_attention_workspace bytes for the same cache, batch sizes and
- * query heads (0: none is needed, or an argument is wrong), 16-byte aligned,
- * zero-filled before its first use and then left to these calls, one at a
- * time (of any batch that it is large enough for). */
+ * is not finite makes the rows that see its block not finite (scales are not
+ * negative). f32 out is computed to f32 rounding. f16 and bf16 out have the
+ * softmax weights rounded to f16 (11 bits down to 2^-21 of the largest weight,
+ * fewer down to 2^-31), and may have f32 queries rounded to f16, each row by a
+ * power of two to below 2 first: over E4M3 codes, and where sequences have
+ * more than 16 rows a kv head. The workspace holds the partial sums of
+ * sequences split over the GPU: at least ditch_cuda_kv_attention_workspace
+ * bytes for the same cache, batch sizes and query heads (0: none is needed, or
+ * an argument is wrong), 16-byte aligned, zero-filled before its first use and
+ * then left to these calls, one at a time (of any batch that it is large
+ * enough for). */
 size_t ditch_cuda_kv_attention_workspace(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache,
                                          const ditch_cuda_kv_batch *batch, size_t q_heads);
 int ditch_cuda_kv_attention(ditch_cuda_device *dev, const ditch_cuda_kv_cache *cache, const ditch_cuda_kv_batch *batch,
